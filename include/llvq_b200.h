@@ -218,6 +218,48 @@ int llvq_hadamard_ex(const void* in, int32_t in_type, void* out, int32_t out_typ
 int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_t ld, int32_t block,
                       const int8_t* signs, float* out, uint16_t* row_scale_out, void* stream);
 
+/* ---- 8-bit operators (no reference counterpart).  An 8-bit matrix is e4m3
+ * bytes in rows of 128-column blocks with fp32 scales: value = byte * scale of
+ * its block; the last block of a row may be partial.  Scales lie anywhere:
+ * scale[r * scale_row + b * scale_col] for row (or row block) r and column
+ * block b.  For each block amax = max(2^-100, max |y|), scale = amax / 448,
+ * byte = e4m3(448 y / amax), the quotient correctly rounded in fp32 and then
+ * to e4m3 (ties to even).  NaN makes its whole block NaN; an infinity makes
+ * the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
+ * have a stride in elements, e4m3 output rows start on 8-byte boundaries (base
+ * and stride).  Device: the current one.  Nothing is allocated and no call
+ * keeps state, so calls may overlap on any streams and be captured. */
+
+/* x [rows, cols] -> q, scales of 1 x 128 blocks (block_rows = 1, activations)
+ * or 128 x 128 blocks (block_rows = 128, weights). */
+int llvq_fp8_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int64_t cols, int32_t block_rows,
+                      uint8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_col, void* stream);
+/* y = gate / (1 + exp(-gate)) * up in fp32, quantized in 1 x 128 blocks. */
+int llvq_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int32_t type, int64_t rows,
+                    int64_t cols, uint8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_col,
+                    void* stream);
+/* h = x + residual in fp32 (residual NULL: h = x), hidden = h rounded once to
+ * `type` (NULL without a residual; must not alias the inputs), y = h *
+ * weight / sqrt(mean(h^2) + eps) per row, quantized in 1 x 128 blocks.  The
+ * norm uses the unrounded h; the sum of squares is fp32 in a fixed order.
+ * weight [cols] has the input's type or fp32. */
+#define LLVQ_FP8_NORM_MAX_COLS 32768
+int llvq_fp8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ld_residual, int32_t type,
+                      const void* weight, int32_t weight_type, float eps, int64_t rows, int64_t cols, void* hidden,
+                      int64_t ld_hidden, uint8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_col,
+                      void* stream);
+/* y[m, n] = sum over column blocks b of a_scale[m, b] w_scale[n / 128, b] *
+ * sum_{k in b} a[m, k] w[n, k]: each block's sum on the tensor cores, scaled
+ * and added in fp32, rounded once to y_type.  a [m, k] with 1 x 128 scales, w
+ * [n, k] with 128 x 128 scales; e4m3 rows start on 16-byte boundaries (base
+ * and stride), y has row stride ldy.  k = 0 gives zeros.  One summation order
+ * per output and shape.  *error_flag (device int, may be NULL) is set to 1 if
+ * a tensor-core wait timed out. */
+int llvq_fp8_gemm(const uint8_t* a, int64_t lda, const float* a_scale, int64_t a_scale_row, int64_t a_scale_col,
+                  const uint8_t* w, int64_t ldw, const float* w_scale, int64_t w_scale_row, int64_t w_scale_col,
+                  int64_t m, int64_t n, int64_t k, void* y, int64_t ldy, int32_t y_type, int32_t* error_flag,
+                  void* stream);
+
 /* Host-side scalar paths (no GPU needed).
  * llvq_codeword_host:  LeechLatticeVectorQuantizerGpu.codeword (_gpu.py:262-265)
  * llvq_encode_host:    LeechLatticeVectorQuantizer.encode_codeword (CPU module :247-280) */

@@ -39,7 +39,8 @@ EXPORTS = (
     "llvq_encode_host", "llvq_status_string", "llvq_last_error", "llvq_version", "llvq_gemm",
     "llvq_hadamard", "llvq_gemm_noalloc", "llvq_pack_indices", "llvq_unpack_indices", "llvq_dequantize_packed",
     "llvq_gemm_packed", "llvq_hadamard_ex", "llvq_codeword_batch_host", "llvq_codebook_tables",
-    "llvq_quantize_gain", "llvq_rotate_scale",
+    "llvq_quantize_gain", "llvq_rotate_scale", "llvq_fp8_quantize", "llvq_fp8_swiglu", "llvq_fp8_rms_norm",
+    "llvq_fp8_gemm",
 )
 
 _lib = None
@@ -78,6 +79,12 @@ def load() -> ctypes.CDLL:
             "llvq_unpack_indices": (ctypes.c_int, [vp, i64, i32, vp, vp]),
             "llvq_dequantize_packed": (ctypes.c_int, [vp, vp, i32, i64, vp, i32, vp, i64, vp, vp]),
             "llvq_gemm_packed": (ctypes.c_int, [vp, vp, i32, i64, i64, vp, vp, i64, i64, vp, vp, vp]),
+            "llvq_fp8_quantize": (ctypes.c_int, [vp, i32, i64, i64, i64, i32, vp, i64, vp, i64, i64, vp]),
+            "llvq_fp8_swiglu": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i64, vp, i64, vp, i64, i64, vp]),
+            "llvq_fp8_rms_norm": (ctypes.c_int, [vp, i64, vp, i64, i32, vp, i32, ctypes.c_float, i64, i64, vp, i64,
+                                                 vp, i64, vp, i64, i64, vp]),
+            "llvq_fp8_gemm": (ctypes.c_int, [vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i64, vp, i64,
+                                             i32, vp, vp]),
             "llvq_codeword_host": (ctypes.c_int, [vp, i64, vp]),
             "llvq_codeword_batch_host": (ctypes.c_int, [vp, vp, i64, vp, P(i64)]),
             "llvq_codebook_tables": (ctypes.c_int, [vp, P(i32), P(i64), P(i32)]),
@@ -246,6 +253,34 @@ def hadamard_ex(in_ptr: int, in_type: int, out_ptr: int, out_type: int, rows: in
                 signs_ptr: int, inverse: bool, stream: int) -> None:
     check(load().llvq_hadamard_ex(in_ptr, in_type, out_ptr, out_type, rows, cols, block, signs_ptr, int(inverse),
                                   stream), "llvq_hadamard_ex")
+
+
+def fp8_quantize(x_ptr: int, x_type: int, ldx: int, rows: int, cols: int, block_rows: int, q_ptr: int, ldq: int,
+                 scale_ptr: int, scale_row: int, scale_col: int, stream: int) -> None:
+    check(load().llvq_fp8_quantize(x_ptr, x_type, ldx, rows, cols, block_rows, q_ptr, ldq, scale_ptr, scale_row,
+                                   scale_col, stream), "llvq_fp8_quantize")
+
+
+def fp8_swiglu(gate_ptr: int, ld_gate: int, up_ptr: int, ld_up: int, dtype: int, rows: int, cols: int, q_ptr: int,
+               ldq: int, scale_ptr: int, scale_row: int, scale_col: int, stream: int) -> None:
+    check(load().llvq_fp8_swiglu(gate_ptr, ld_gate, up_ptr, ld_up, dtype, rows, cols, q_ptr, ldq, scale_ptr,
+                                 scale_row, scale_col, stream), "llvq_fp8_swiglu")
+
+
+def fp8_rms_norm(x_ptr: int, ldx: int, residual_ptr: int, ld_residual: int, dtype: int, weight_ptr: int,
+                 weight_type: int, eps: float, rows: int, cols: int, hidden_ptr: int, ld_hidden: int, q_ptr: int,
+                 ldq: int, scale_ptr: int, scale_row: int, scale_col: int, stream: int) -> None:
+    check(load().llvq_fp8_rms_norm(x_ptr, ldx, residual_ptr, ld_residual, dtype, weight_ptr, weight_type, eps, rows,
+                                   cols, hidden_ptr, ld_hidden, q_ptr, ldq, scale_ptr, scale_row, scale_col, stream),
+          "llvq_fp8_rms_norm")
+
+
+def fp8_gemm(a_ptr: int, lda: int, a_scale_ptr: int, a_scale_row: int, a_scale_col: int, w_ptr: int, ldw: int,
+             w_scale_ptr: int, w_scale_row: int, w_scale_col: int, m: int, n: int, k: int, y_ptr: int, ldy: int,
+             y_type: int, flag_ptr: int, stream: int) -> None:
+    check(load().llvq_fp8_gemm(a_ptr, lda, a_scale_ptr, a_scale_row, a_scale_col, w_ptr, ldw, w_scale_ptr,
+                               w_scale_row, w_scale_col, m, n, k, y_ptr, ldy, y_type, flag_ptr, stream),
+          "llvq_fp8_gemm")
 
 
 def rotate_scale(in_ptr: int, rows: int, cols: int, ld: int, block: int, signs_ptr: int, out_ptr: int,

@@ -935,3 +935,23 @@ const char* llvq_last_error(void) { return g_last_error.c_str(); }
 int llvq_version(void) { return 1; }
 
 }  // extern "C"
+
+namespace llvq {
+
+int abi_error(int status, const char* msg) noexcept {
+  try {
+    return fail(status, msg);
+  } catch (...) {  // no memory for the message: the status stands
+    return status;
+  }
+}
+
+int abi_cuda_error(cudaError_t e, const char* where) noexcept {
+  try {
+    return cuda_fail(e, where);
+  } catch (...) {
+    return LLVQ_ERR_CUDA;
+  }
+}
+
+}  // namespace llvq

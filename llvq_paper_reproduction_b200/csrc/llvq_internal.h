@@ -161,4 +161,50 @@ cudaError_t rotate_scale_launch(const void* in, int64_t rows, int64_t cols, int6
 cudaError_t hadamard_launch(const void* in, int in_type, void* out, int out_type, int64_t rows, int64_t cols,
                             int block, const int8_t* signs, int inverse, cudaStream_t stream);
 
+// 8-bit operators (fp8_quant.cu, fp8_gemm.cu): e4m3 values with one fp32
+// scale per block of 128 columns.  Element types: LLVQ_DT_*.
+constexpr int kFp8Block = 128;
+constexpr int64_t kFp8NormMaxCols = 32768;  // a row of the norm stays in the registers of one CTA
+
+// Where a quantizer writes: e4m3 rows (row stride ld, a multiple of 8, base
+// 8-byte aligned) and the scale of row (or row block) r and column block b at
+// scale[r * scale_row + b * scale_col].
+struct Fp8Out {
+  uint8_t* q;
+  int64_t ld;
+  float* scale;
+  int64_t scale_row, scale_col;
+};
+
+// An input matrix: row stride ld in elements.
+struct Fp8In {
+  const void* ptr;
+  int64_t ld;
+};
+
+cudaError_t fp8_quantize_launch(Fp8In x, int type, int64_t rows, int64_t cols, int block_rows, Fp8Out out,
+                                cudaStream_t stream);
+cudaError_t fp8_swiglu_launch(Fp8In gate, Fp8In up, int type, int64_t rows, int64_t cols, Fp8Out out,
+                              cudaStream_t stream);
+// residual.ptr and hidden may be null (both or neither).
+cudaError_t fp8_rms_norm_launch(Fp8In x, Fp8In residual, int type, const void* weight, int weight_type, float eps,
+                                int64_t rows, int64_t cols, void* hidden, int64_t ld_hidden, Fp8Out out,
+                                cudaStream_t stream);
+
+// An e4m3 operand of the product with its scales (strides in elements; ld a
+// multiple of 16, q 16-byte aligned).
+struct Fp8Operand {
+  const uint8_t* q;
+  int64_t ld;
+  const float* scale;
+  int64_t scale_row, scale_col;
+};
+
+cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,
+                            int y_type, int* error_flag, cudaStream_t stream);
+
+// Status and message of the C entry points outside codebook.cu.
+int abi_error(int status, const char* msg) noexcept;
+int abi_cuda_error(cudaError_t e, const char* where) noexcept;
+
 }  // namespace llvq

@@ -244,6 +244,25 @@ class LeechLatticeVectorQuantizerGpu:
             self.raise_pending_errors()
         return out
 
+    def dequantize_fp8(self, indices: torch.Tensor, row_scale: torch.Tensor, cols: int | None = None,
+                       check: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+        """The weight of ``gemm`` laid out once for the 8-bit product: e4m3
+        [rows, cols] and fp32 scales [ceil(rows / 128), ceil(cols / 128)]
+        (``fp8.quantize_blocks`` of ``dequantize_bf16``), where cols cuts the
+        padding of the last block off (default: all 24 * blocks columns).
+        Against the dequant-GEMM it takes a byte instead of 2 bits per weight
+        and rounds the weight to 3 fraction bits, and gives large batches
+        the 8-bit tensor rate.  Errors as in ``dequantize_bf16``.  No
+        reference counterpart."""
+        from . import fp8
+
+        w = self.dequantize_bf16(indices, row_scale, check=check)
+        if cols is not None:
+            if not 0 <= cols <= w.shape[1]:
+                raise ValueError(f"cols must be in 0..{w.shape[1]}")
+            w = w[:, :cols]
+        return fp8.quantize_blocks(w)
+
     def gemm(self, a: torch.Tensor, indices: torch.Tensor, row_scale: torch.Tensor | None = None,
              rotation: tuple[int, torch.Tensor] | None = None, check: bool = False) -> torch.Tensor:
         """Dequant-GEMM: ``a @ W.T`` in fp32 for bf16 activations ``a`` [m, k]
