@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -27,59 +28,118 @@ namespace llvq {
 
 namespace {
 
-constexpr int kVec = 8;                          // elements a thread handles at a time
-constexpr int kGroup = kFp8Block / kVec;         // 16 threads share one block of 128 columns
+constexpr int kVec = 16;                         // elements a thread handles at a time
+constexpr int kGroup = kFp8Block / kVec;         // 8 threads share one block of 128 columns
 constexpr float kE4m3Max = 448.f;
 constexpr float kAmaxFloor = 0x1p-100f;
 
+// Sixteen elements as they lie in memory: pairs of 16-bit values, or fp32.
 template <typename T>
-__device__ __forceinline__ float to_float(T v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else return static_cast<float>(v);
-}
-
-template <typename T>
-__device__ __forceinline__ T from_float(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
-  else return __float2bfloat16_rn(v);
-}
-
-// Eight elements as they lie in memory.
-template <typename T>
-struct alignas(16) Raw {
-  T v[kVec];
+struct Raw {
+  static constexpr int kWords = kVec * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
 };
 
-// kAligned: every full group of eight starts on a 16-byte boundary.
-template <typename T, bool kAligned>
-__device__ __forceinline__ Raw<T> load8(const T* p, int valid) {
-  Raw<T> r;
-  if (kAligned && valid >= kVec) {
-    const uint4* s = reinterpret_cast<const uint4*>(p);
-    uint4* d = reinterpret_cast<uint4*>(&r);
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[kVec]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(r) / 16); ++i) d[i] = __ldg(s + i);
+    for (int i = 0; i < kVec; ++i) v[i] = __uint_as_float(r.w[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) r.v[i] = i < valid ? p[i] : from_float<T>(0.f);
+    for (int i = 0; i < kVec / 2; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(r.w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> pack(const float (&v)[kVec]) {
+  Raw<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) r.w[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        r.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
   }
   return r;
 }
 
-template <typename T, bool kAligned>
-__device__ __forceinline__ void store8(T* p, const Raw<T>& r, int valid) {
-  if (kAligned && valid >= kVec) {
-    uint4* d = reinterpret_cast<uint4*>(p);
-    const uint4* s = reinterpret_cast<const uint4*>(&r);
+// Sixteen elements, those from `valid` on as zeros.  kStep elements are loaded
+// at a time (8 or 4: every step starts on its boundary, 16 bytes at most, and
+// the columns are a multiple of it; 1: nothing is known), by predicated loads
+// without branches, so that all the loads of a thread are in flight together.
+template <typename T, int kStep>
+__device__ __forceinline__ Raw<T> load_vec(const T* p, int valid) {
+  Raw<T> r;
+  if constexpr (kStep * sizeof(T) >= 16) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(r) / 16); ++i) d[i] = s[i];
+    for (int i = 0; i < Raw<T>::kWords / 4; ++i) {
+      const bool in = i * 16 < valid * (int)sizeof(T);
+      const uint4 q = in ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+      r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+    }
+  } else if constexpr (kStep * sizeof(T) == 8) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords / 2; ++i) {
+      const bool in = i * 8 < valid * (int)sizeof(T);
+      const uint2 q = in ? __ldg(reinterpret_cast<const uint2*>(p) + i) : make_uint2(0, 0);
+      r.w[2 * i] = q.x, r.w[2 * i + 1] = q.y;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) r.w[i] = i < valid ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+  } else {
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+      const uint32_t lo = 2 * i < valid ? __ldg(s + 2 * i) : 0u, hi = 2 * i + 1 < valid ? __ldg(s + 2 * i + 1) : 0u;
+      r.w[i] = lo | hi << 16;
+    }
+  }
+  return r;
+}
+
+template <typename T, int kStep>
+__device__ __forceinline__ void store_vec(T* p, const Raw<T>& r, int valid) {
+  if constexpr (kStep * sizeof(T) >= 16) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords / 4; ++i)
+      if (i * 16 < valid * (int)sizeof(T))
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+  } else if constexpr (kStep * sizeof(T) == 8) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords / 2; ++i)
+      if (i * 8 < valid * (int)sizeof(T)) reinterpret_cast<uint2*>(p)[i] = make_uint2(r.w[2 * i], r.w[2 * i + 1]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (i < valid) reinterpret_cast<uint32_t*>(p)[i] = r.w[i];
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
-      if (i < valid) p[i] = r.v[i];
+      if (i < valid) reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(r.w[i / 2] >> (16 * (i & 1)));
   }
 }
+
+__device__ __forceinline__ float2 both(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 both(__nv_bfloat162 v) { return __bfloat1622float2(v); }
 
 // max |.| that keeps NaN (fmaxf would drop it).
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -88,39 +148,99 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float amax8(const float (&v)[kVec]) {
+__device__ __forceinline__ float amax_of(const float (&v)[kVec]) {
   float m = fabsf(v[0]);
 #pragma unroll
   for (int i = 1; i < kVec; ++i) m = max_nan(m, fabsf(v[i]));
   return m;
 }
 
-// Largest of the 16 threads that share a block (a half warp).
+// The same of the values as they lie in memory: pairs at a time (their largest
+// magnitude is one of them, so nothing is rounded).
+template <typename T>
+__device__ __forceinline__ float amax_of(const Raw<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    float v[kVec];
+    unpack(r, v);
+    return amax_of(v);
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 m = __habs2(*reinterpret_cast<const T2*>(&r.w[0]));
+#pragma unroll
+    for (int i = 1; i < Raw<T>::kWords; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&r.w[i])));
+    const float2 f = both(m);
+    return max_nan(f.x, f.y);
+  }
+}
+
+// Largest of the 8 threads that share a block.
 __device__ __forceinline__ float group_max(float m) {
 #pragma unroll
   for (int o = kGroup / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
 
-// 448 v / amax correctly rounded, from the reciprocal r = RN(1 / amax) and one
-// residual step (Markstein 1990: q0 = z r, q = q0 + (z - q0 amax) r).  The
-// multiplier 448 and amax are both taken times 2^-64 where 448 amax could
+__device__ __forceinline__ float floored(float amax) { return max_nan(amax, kAmaxFloor); }
+
+// RN(amax / 448): one residual step from the rounded reciprocal (Markstein 1990).
+__device__ __forceinline__ float scale_of(float amax) {
+  constexpr float kInv = 1.f / kE4m3Max;
+  const float q = amax * kInv;
+  return isinf(q) ? q : fmaf(fmaf(-q, kE4m3Max, amax), kInv, q);
+}
+
+// 1 / d within one unit: the approximate reciprocal and a Newton step (d normal, not near the ends of the range).
+__device__ __forceinline__ float reciprocal(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return fmaf(r, fmaf(-d, r, 1.f), r);
+}
+
+// 1 / sqrt(v) within two units, from the approximate root and a Newton step;
+// infinite for 0, 0 for infinity.
+__device__ __forceinline__ float inverse_root(float v) {
+  float r;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  const float better = fmaf(fmaf(-v * r, r, 1.f), 0.5f * r, r);
+  return v > 0x1p-126f && v < 0x1p126f ? better : r;
+}
+
+// 448 v / amax for values v that fp32 holds exactly: q0 = z r with z = 448 v
+// (exact for 16-bit inputs) and r = 1 / amax, and one residual step, q = q0 +
+// (z - q0 amax) r (Markstein 1990).  Inputs of few bits lie on ties of e4m3
+// often, and there the residual is exact and q is the tie itself, so that it
+// is rounded to even as it should; a quotient off by one unit would fall on
+// either side.  448 and amax are both taken times 2^-64 where 448 amax could
 // overflow; an infinite amax gives 0 for finite values and NaN for infinite ones.
-struct Quotient {
+struct ExactQuotient {
   float mul, d, r, scale;
-  __device__ __forceinline__ explicit Quotient(float amax) {
-    amax = max_nan(amax, kAmaxFloor);
-    scale = __fdiv_rn(amax, kE4m3Max);
+  __device__ __forceinline__ explicit ExactQuotient(float amax) {
+    amax = floored(amax);
+    scale = scale_of(amax);
     const bool big = amax > 0x1p100f;
     mul = big ? kE4m3Max * 0x1p-64f : kE4m3Max;
     d = big ? amax * 0x1p-64f : amax;
-    r = __frcp_rn(d);
-    if (isinf(amax)) d = 0.f;
+    r = reciprocal(d);
+    if (isinf(amax)) d = r = 0.f;
   }
   __device__ __forceinline__ float operator()(float v) const {
     const float z = v * mul, q = z * r;
     return fmaf(fmaf(-q, d, z), r, q);
   }
+};
+
+// 448 v / amax for values that carry fp32 roundings themselves: one product
+// with 448 / amax.
+struct Quotient {
+  float r, scale;
+  __device__ __forceinline__ explicit Quotient(float amax) {
+    amax = floored(amax);
+    scale = scale_of(amax);
+    const bool big = amax > 0x1p100f;
+    r = reciprocal(big ? amax * 0x1p-64f : amax) * (big ? kE4m3Max * 0x1p-64f : kE4m3Max);
+    if (isinf(amax)) r = 0.f;
+  }
+  __device__ __forceinline__ float operator()(float v) const { return v * r; }
 };
 
 // Two e4m3 bytes, lo in the low one.
@@ -130,13 +250,15 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ void store_q8(uint8_t* p, const float (&v)[kVec], const Quotient& quo, int valid) {
-  uint32_t w[2];
+// Sixteen values as e4m3; rows start on 16-byte boundaries.
+template <typename Q>
+__device__ __forceinline__ void store_q(uint8_t* p, const float (&v)[kVec], const Q& quo, int valid) {
+  uint32_t w[kVec / 4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < kVec / 4; ++i)
     w[i] = e4m3x2(quo(v[4 * i]), quo(v[4 * i + 1])) | e4m3x2(quo(v[4 * i + 2]), quo(v[4 * i + 3])) << 16;
   if (valid >= kVec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
@@ -149,48 +271,87 @@ __device__ __forceinline__ int valid_of(int64_t cols, int64_t c) {
   return left >= kVec ? kVec : left > 0 ? (int)left : 0;
 }
 
-// ---------------------------------------------------------------- rows
-// One half warp per (row, block of 128 columns): a thread's eight elements
-// are 16 bytes of a 16-bit input, and consecutive half warps read consecutive
-// blocks, so every access is whole lines.  kGated: y = gate / (1 + exp(-gate)) * up.
-constexpr int kRowThreads = 256;
+// gate / (1 + exp(-gate)).  exp(-g) = 2^h (1 + l ln 2), h = RN(-g kLog2e) and l
+// what that product and the rounded constant lost (kLog2e = log2 e - 1.926e-8,
+// kTail = -1.926e-8 ln 2), so that its error is that of ex2.approx (2^-22) for
+// every g; the reciprocal takes one Newton step.  Below g = -87.3 the
+// reciprocal is flushed to zero, the quotient g * 0 (NaN for an infinite g).
+__device__ __forceinline__ float silu(float g) {
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kTail = -1.33497582e-8f;
+  const float c = fmaxf(g, -88.5f);  // 2^h stays finite
+  const float h = c * -kLog2e;
+  const float l = fmaf(c, -kLog2e, -h);
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
+  e = fmaf(e, fmaf(c, kTail, l * kLn2), e);
+  return g * reciprocal(1.f + e);
+}
 
-template <typename T, bool kGated, bool kAligned>
+// ---------------------------------------------------------------- rows
+// Eight threads per (row, block of 128 columns), the next eight on the next
+// block, so that every line is read and written whole; a thread loads all its
+// kUnits units before it works on the first.  Sixteen elements a thread, not
+// eight: what a thread spends once on a unit (three shuffles, the quotient, the
+// addresses) was half of its instructions.  kGated: y = gate / (1 + exp(-gate)) * up.
+constexpr int kRowThreads = 256;
+template <typename T, bool kGated>
+constexpr int kRowUnits = kGated || sizeof(T) == 4 ? 1 : 2;
+
+template <typename T, bool kGated, int kStep>
 __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* __restrict__ x, int64_t ldx,
-                                                           const T* __restrict__ up, int64_t ldu, uint32_t units,
-                                                           uint32_t blocks, int64_t cols, Fp8Out out) {
-  const uint32_t u = blockIdx.x * (kRowThreads / kGroup) + threadIdx.x / kGroup;
-  const bool live = u < units;  // no early return: the whole warp meets in the shuffles
-  const uint32_t row = live ? u / blocks : 0, b = live ? u % blocks : 0;
-  const int64_t c = (int64_t)b * kFp8Block + (threadIdx.x % kGroup) * kVec;
-  const int valid = live ? valid_of(cols, c) : 0;
-  const Raw<T> rx = load8<T, kAligned>(x + row * ldx + c, valid);
-  float v[kVec];
-  if constexpr (kGated) {
-    const Raw<T> ru = load8<T, kAligned>(up + row * ldu + c, valid);
+                                                           const T* __restrict__ up, int64_t ldu, uint32_t rows,
+                                                           uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
+                                                           int64_t cols, Fp8Out out) {
+  constexpr int kUnits = kRowUnits<T, kGated>;
+  constexpr int kTeams = kRowThreads / kGroup;
+  const uint32_t first = blockIdx.x * (kTeams * kUnits) + threadIdx.x / kGroup;
+  const int in_block = (int)(threadIdx.x % kGroup) * kVec;
+  uint32_t row[kUnits], b[kUnits];
+  int valid[kUnits];
+  Raw<T> rx[kUnits], ru[kUnits];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const float g = to_float(rx.v[i]);
-      v[i] = __fdiv_rn(g, 1.f + expf(-g)) * to_float(ru.v[i]);
+  for (int j = 0; j < kUnits; ++j) {
+    if (j == 0) {
+      row[0] = first / blocks;
+      b[0] = first - row[0] * blocks;
+    } else {  // kTeams units on: skip_rows rows and skip_blocks blocks, without another division
+      const uint32_t next = b[j - 1] + skip_blocks, wrap = next >= blocks;
+      row[j] = row[j - 1] + skip_rows + wrap;
+      b[j] = wrap ? next - blocks : next;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = to_float(rx.v[i]);
+    const int64_t c = (int64_t)b[j] * kFp8Block + in_block;
+    valid[j] = row[j] < rows ? valid_of(cols, c) : 0;  // no early return: the whole warp meets in the shuffles
+    rx[j] = load_vec<T, kStep>(x + (valid[j] ? row[j] * ldx + c : 0), valid[j]);
+    if constexpr (kGated) ru[j] = load_vec<T, kStep>(up + (valid[j] ? row[j] * ldu + c : 0), valid[j]);
   }
-  const Quotient quo(group_max(amax8(v)));
-  if (!live) return;
-  store_q8(out.q + row * out.ld + c, v, quo, valid);
-  if (threadIdx.x % kGroup == 0) out.scale[row * out.scale_row + b * out.scale_col] = quo.scale;
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    float v[kVec], largest;
+    unpack(rx[j], v);
+    if constexpr (kGated) {
+      float w[kVec];
+      unpack(ru[j], w);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[i] = silu(v[i]) * w[i];
+      largest = amax_of(v);
+    } else {
+      largest = amax_of(rx[j]);
+    }
+    const std::conditional_t<kGated, Quotient, ExactQuotient> quo(group_max(largest));
+    if (!valid[j]) continue;
+    store_q(out.q + row[j] * out.ld + (int64_t)b[j] * kFp8Block + in_block, v, quo, valid[j]);
+    if (in_block == 0) out.scale[row[j] * out.scale_row + b[j] * out.scale_col] = quo.scale;
+  }
 }
 
 // ---------------------------------------------------------------- 128 x 128 blocks
 // One CTA per block: 256 threads hold its 16,384 values in registers (64 per
 // thread, as they lie in memory) between the maximum and the store.
 constexpr int kBlockThreads = 256;
-constexpr int kBlockRowsPass = kBlockThreads / kGroup;       // 16 rows a pass
-constexpr int kBlockPasses = kFp8Block / kBlockRowsPass;     // 8
+constexpr int kBlockRowsPass = kBlockThreads / kGroup;       // 32 rows a pass
+constexpr int kBlockPasses = kFp8Block / kBlockRowsPass;     // 4
 
-template <typename T, bool kAligned>
+template <typename T, int kStep>
 __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                                int64_t cols, uint32_t col_blocks, Fp8Out out) {
   __shared__ float red[kBlockThreads / 32];
@@ -202,118 +363,139 @@ __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* __restri
 #pragma unroll
   for (int p = 0; p < kBlockPasses; ++p) {
     const int64_t r = r0 + p * kBlockRowsPass;
-    raw[p] = load8<T, kAligned>(x + (r < rows ? r * ldx + c : 0), r < rows ? valid : 0);
+    const int live = r < rows ? valid : 0;
+    raw[p] = load_vec<T, kStep>(x + (live ? r * ldx + c : 0), live);
   }
   float m = 0.f;
 #pragma unroll
-  for (int p = 0; p < kBlockPasses; ++p) {
-    float v[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = to_float(raw[p].v[i]);
-    m = max_nan(m, amax8(v));
-  }
+  for (int p = 0; p < kBlockPasses; ++p) m = max_nan(m, amax_of(raw[p]));
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kBlockThreads / 32; ++w) m = max_nan(m, red[w]);
-  const Quotient quo(m);
+  const ExactQuotient quo(m);
 #pragma unroll
   for (int p = 0; p < kBlockPasses; ++p) {
     const int64_t r = r0 + p * kBlockRowsPass;
-    if (r < rows) {
+    if (r < rows && valid) {
       float v[kVec];
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) v[i] = to_float(raw[p].v[i]);
-      store_q8(out.q + r * out.ld + c, v, quo, valid);
+      unpack(raw[p], v);
+      store_q(out.q + r * out.ld + c, v, quo, valid);
     }
   }
   if (threadIdx.x == 0) out.scale[rb * out.scale_row + cb * out.scale_col] = quo.scale;
 }
 
 // ---------------------------------------------------------------- RMS norm
-// One CTA per row; the row stays in registers (kChunks groups of eight per
-// thread) between the sum of squares and the 8-bit store:
+// A CTA takes rows blockIdx.x, + gridDim.x, ...; a row stays in registers
+// (kChunks groups of sixteen per thread) between the sum of squares and the 8-bit
+// store, and the next row's loads are under way meanwhile:
 //   h = x + residual (fp32; hidden = h rounded once)    y = h rsqrt(mean h^2 + eps) weight
 // The norm uses the unrounded sum h.  Threads past the row hold zeros.
-// One chunk up to 512 threads, more chunks up to 1024 (64 registers each).
-template <int kChunks>
-constexpr int kNormThreads = kChunks == 1 ? 512 : 1024;
-
-template <typename T, typename W, int kChunks, bool kResidual, bool kAligned>
-__global__ void __launch_bounds__(kNormThreads<kChunks>) rms_norm_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ residual, int64_t ldr,
-                                const W* __restrict__ weight, float eps, int64_t cols, T* __restrict__ hidden,
-                                int64_t ldh, Fp8Out out) {
-  __shared__ float red[32];
-  const int64_t row = blockIdx.x;
-  float h[kChunks][kVec];
+// Three shapes: up to 8192 columns one chunk, up to 16,384 two, with at most 512
+// threads and the next row in registers; beyond, two chunks of up to 1024
+// threads, which leave no registers for it.  (One chunk of 688 threads, for 11008
+// columns, left an SM with a single CTA: 63 us against the two chunks' 56 for
+// 4096 rows.)
+template <typename T, typename W, int kChunks, int kThreads, bool kResidual, int kStep>
+__global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 80 : 64)
+    rms_norm_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ residual, int64_t ldr,
+                    const W* __restrict__ weight, float eps, float inv_cols, int64_t rows, int64_t cols,
+                    T* __restrict__ hidden, int64_t ldh, Fp8Out out) {
+  constexpr bool kAhead = kThreads == 512 && sizeof(T) == 2;  // fp32 rows would spill
+  __shared__ float red[2][32];
   Raw<T> rx[kChunks], rr[kChunks];
-  Raw<W> rw[kChunks];
+  auto load = [&](int64_t row) {
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
-    const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
-    const int valid = valid_of(cols, c);
-    rx[j] = load8<T, kAligned>(x + row * ldx + c, valid);
-    if constexpr (kResidual) rr[j] = load8<T, kAligned>(residual + row * ldr + c, valid);
-    rw[j] = load8<W, kAligned>(weight + c, valid);
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
-    const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
-    Raw<T> rh;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      h[j][i] = to_float(rx[j].v[i]);
-      if constexpr (kResidual) {
-        h[j][i] += to_float(rr[j].v[i]);
-        rh.v[i] = from_float<T>(h[j][i]);
-      }
-      ss = fmaf(h[j][i], h[j][i], ss);
+    for (int j = 0; j < kChunks; ++j) {
+      const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
+      const int valid = row < rows ? valid_of(cols, c) : 0;
+      rx[j] = load_vec<T, kStep>(x + (valid ? row * ldx + c : 0), valid);
+      if constexpr (kResidual) rr[j] = load_vec<T, kStep>(residual + (valid ? row * ldr + c : 0), valid);
     }
-    if constexpr (kResidual) store8<T, kAligned>(hidden + row * ldh + c, rh, valid_of(cols, c));
-  }
+  };
+  if constexpr (kAhead) load(blockIdx.x);
+  int side = 0;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, side ^= 1) {
+    float h[kChunks][kVec];
+    float ss = 0.f;
+    if constexpr (!kAhead) load(row);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  float total = 0.f;
-  for (unsigned w = 0; w < blockDim.x / 32; ++w) total += red[w];
-  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(total, (float)cols) + eps));
+    for (int j = 0; j < kChunks; ++j) {
+      unpack(rx[j], h[j]);
+      if constexpr (kResidual) {
+        float r[kVec];
+        unpack(rr[j], r);
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
-    const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
-    const int valid = valid_of(cols, c);
-    float y[kVec];
+        for (int i = 0; i < kVec; ++i) h[j][i] += r[i];
+      }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) y[i] = valid > i ? h[j][i] * rstd * to_float(rw[j].v[i]) : 0.f;
-    const Quotient quo(group_max(amax8(y)));
-    store_q8(out.q + row * out.ld + c, y, quo, valid);
-    if (threadIdx.x % kGroup == 0 && valid > 0)
-      out.scale[row * out.scale_row + c / kFp8Block * out.scale_col] = quo.scale;
+      for (int i = 0; i < kVec; ++i) ss = fmaf(h[j][i], h[j][i], ss);
+    }
+    if constexpr (kAhead) load(row + gridDim.x);
+    if constexpr (kResidual) {
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
+        const int valid = valid_of(cols, c);
+        store_vec<T, kStep>(hidden + (valid ? row * ldh + c : 0), pack<T>(h[j]), valid);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if ((threadIdx.x & 31) == 0) red[side][threadIdx.x >> 5] = ss;
+    __syncthreads();  // the other side is written next: one barrier a row
+    // every warp adds the warps' sums in the same tree
+    float total = (threadIdx.x & 31) < blockDim.x / 32 ? red[side][threadIdx.x & 31] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float var = fmaf(total, inv_cols, eps);
+    const float rstd = inverse_root(var);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
+      const int valid = valid_of(cols, c);
+      const Raw<W> rw = load_vec<W, kStep>(weight + (valid ? c : 0), valid);
+      float y[kVec];
+      unpack(rw, y);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) y[i] = h[j][i] * rstd * y[i];
+      const Quotient quo(group_max(amax_of(y)));
+      if (valid) store_q(out.q + row * out.ld + c, y, quo, valid);
+      if (valid && threadIdx.x % kGroup == 0)
+        out.scale[row * out.scale_row + c / kFp8Block * out.scale_col] = quo.scale;
+    }
   }
 }
 
+// The elements of a matrix that can be loaded at a time: 8, 4 or 1 (load_vec).
 template <typename T>
-bool aligned16(const void* p, int64_t ld) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
+int step_of(const void* p, int64_t ld, int64_t cols) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (int64_t)sizeof(T));
+  const uintptr_t wide = sizeof(T) * 8 > 16 ? 16 : sizeof(T) * 8, half = sizeof(T) * 4;
+  return at % wide == 0 && cols % 8 == 0 ? 8 : at % half == 0 && cols % 4 == 0 ? 4 : 1;
+}
+
+template <typename T, bool kGated, int kStep>
+cudaError_t rows_step(Fp8In x, Fp8In up, int64_t rows, int64_t cols, Fp8Out out, cudaStream_t stream) {
+  const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block, units = rows * blocks;
+  constexpr int kTeams = kRowThreads / kGroup, kCta = kTeams * kRowUnits<T, kGated>;
+  if (units > 0xFFFFFFFFLL - kCta) return cudaErrorInvalidValue;
+  rows_kernel<T, kGated, kStep><<<(unsigned)((units + kCta - 1) / kCta), kRowThreads, 0, stream>>>(
+      static_cast<const T*>(x.ptr), x.ld, static_cast<const T*>(up.ptr), up.ld, (uint32_t)rows, (uint32_t)blocks,
+      (uint32_t)(kTeams / blocks), (uint32_t)(kTeams % blocks), cols, out);
+  return cudaGetLastError();
 }
 
 template <typename T, bool kGated>
 cudaError_t rows_typed(Fp8In x, Fp8In up, int64_t rows, int64_t cols, Fp8Out out, cudaStream_t stream) {
-  const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block, units = rows * blocks;
-  if (units > 0xFFFFFFF0LL) return cudaErrorInvalidValue;
-  const int64_t grid = (units + kRowThreads / kGroup - 1) / (kRowThreads / kGroup);
-  const T *px = static_cast<const T*>(x.ptr), *pu = static_cast<const T*>(up.ptr);
-  const bool ok = aligned16<T>(px, x.ld) && (!kGated || aligned16<T>(pu, up.ld));
-  if (ok)
-    rows_kernel<T, kGated, true><<<(unsigned)grid, kRowThreads, 0, stream>>>(px, x.ld, pu, up.ld, (uint32_t)units,
-                                                                             (uint32_t)blocks, cols, out);
-  else
-    rows_kernel<T, kGated, false><<<(unsigned)grid, kRowThreads, 0, stream>>>(px, x.ld, pu, up.ld, (uint32_t)units,
-                                                                              (uint32_t)blocks, cols, out);
-  return cudaGetLastError();
+  int step = step_of<T>(x.ptr, x.ld, cols);
+  if (kGated) step = std::min(step, step_of<T>(up.ptr, up.ld, cols));
+  if (step == 8) return rows_step<T, kGated, 8>(x, up, rows, cols, out, stream);
+  if (step == 4) return rows_step<T, kGated, 4>(x, up, rows, cols, out, stream);
+  return rows_step<T, kGated, 1>(x, up, rows, cols, out, stream);
 }
 
 template <typename T>
@@ -321,46 +503,63 @@ cudaError_t blocks_typed(Fp8In x, int64_t rows, int64_t cols, Fp8Out out, cudaSt
   const int64_t rb = (rows + kFp8Block - 1) / kFp8Block, cb = (cols + kFp8Block - 1) / kFp8Block;
   if (rb * cb > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
   const T* px = static_cast<const T*>(x.ptr);
-  if (aligned16<T>(px, x.ld))
-    blocks_kernel<T, true><<<(unsigned)(rb * cb), kBlockThreads, 0, stream>>>(px, x.ld, rows, cols, (uint32_t)cb, out);
-  else
-    blocks_kernel<T, false><<<(unsigned)(rb * cb), kBlockThreads, 0, stream>>>(px, x.ld, rows, cols, (uint32_t)cb,
-                                                                               out);
+#define LLVQ_BLOCKS(S) \
+  blocks_kernel<T, S><<<(unsigned)(rb * cb), kBlockThreads, 0, stream>>>(px, x.ld, rows, cols, (uint32_t)cb, out)
+  const int step = step_of<T>(px, x.ld, cols);
+  if (step == 8) LLVQ_BLOCKS(8);
+  else if (step == 4) LLVQ_BLOCKS(4);
+  else LLVQ_BLOCKS(1);
+#undef LLVQ_BLOCKS
   return cudaGetLastError();
 }
 
-template <typename T, typename W, int kChunks>
-cudaError_t norm_chunks(const T* x, int64_t ldx, const T* r, int64_t ldr, const W* w, float eps, int64_t rows,
-                        int64_t cols, T* hidden, int64_t ldh, Fp8Out out, cudaStream_t stream) {
-  const int64_t groups = (cols + kVec - 1) / kVec;
-  const unsigned threads = (unsigned)(((groups + kChunks - 1) / kChunks + 31) / 32 * 32);
-  const bool ok = aligned16<T>(x, ldx) && aligned16<W>(w, 0) &&
-                  (!r || (aligned16<T>(r, ldr) && aligned16<T>(hidden, ldh)));
-#define LLVQ_NORM(R, A) \
-  rms_norm_kernel<T, W, kChunks, R, A><<<(unsigned)rows, threads, 0, stream>>>(x, ldx, r, ldr, w, eps, cols, hidden, \
-                                                                              ldh, out)
-  if (r) {
-    if (ok) LLVQ_NORM(true, true);
-    else LLVQ_NORM(true, false);
-  } else {
-    if (ok) LLVQ_NORM(false, true);
-    else LLVQ_NORM(false, false);
-  }
-#undef LLVQ_NORM
+struct NormCall {
+  Fp8In x, residual;
+  const void* weight;
+  float eps;
+  int64_t rows, cols;
+  void* hidden;
+  int64_t ldh;
+  Fp8Out out;
+  cudaStream_t stream;
+};
+
+template <typename T, typename W, int kChunks, int kThreads, bool kResidual, int kStep>
+cudaError_t norm_step(const NormCall& n) {
+  const int64_t groups = (n.cols + kVec - 1) / kVec;
+  const int threads = (int)(((groups + kChunks - 1) / kChunks + 31) / 32 * 32);
+  const auto kernel = rms_norm_kernel<T, W, kChunks, kThreads, kResidual, kStep>;
+  int sms = 0;
+  const cudaError_t e = device_sms(&sms);
+  if (e != cudaSuccess) return e;
+  const int64_t resident = (int64_t)sms * std::max(1, (kChunks == 1 ? 1024 : 704) / threads);  // one wave
+  kernel<<<(unsigned)std::min(n.rows, resident), threads, 0, n.stream>>>(
+      static_cast<const T*>(n.x.ptr), n.x.ld, static_cast<const T*>(n.residual.ptr), n.residual.ld,
+      static_cast<const W*>(n.weight), n.eps, 1.f / (float)n.cols, n.rows, n.cols,
+      static_cast<T*>(n.hidden), n.ldh, n.out);
   return cudaGetLastError();
+}
+
+template <typename T, typename W, int kChunks, int kThreads>
+cudaError_t norm_chunks(const NormCall& n) {
+  int step = std::min(step_of<T>(n.x.ptr, n.x.ld, n.cols), step_of<W>(n.weight, 0, n.cols));
+  if (n.residual.ptr)
+    step = std::min({step, step_of<T>(n.residual.ptr, n.residual.ld, n.cols), step_of<T>(n.hidden, n.ldh, n.cols)});
+  if (n.residual.ptr) {
+    if (step == 8) return norm_step<T, W, kChunks, kThreads, true, 8>(n);
+    if (step == 4) return norm_step<T, W, kChunks, kThreads, true, 4>(n);
+    return norm_step<T, W, kChunks, kThreads, true, 1>(n);
+  }
+  if (step == 8) return norm_step<T, W, kChunks, kThreads, false, 8>(n);
+  if (step == 4) return norm_step<T, W, kChunks, kThreads, false, 4>(n);
+  return norm_step<T, W, kChunks, kThreads, false, 1>(n);
 }
 
 template <typename T, typename W>
-cudaError_t norm_typed(Fp8In x, Fp8In r, const void* w, float eps, int64_t rows, int64_t cols, void* hidden,
-                       int64_t ldh, Fp8Out out, cudaStream_t stream) {
-  const T *px = static_cast<const T*>(x.ptr), *pr = static_cast<const T*>(r.ptr);
-  T* ph = static_cast<T*>(hidden);
-  const W* pw = static_cast<const W*>(w);
-  if (cols <= 512 * kVec)
-    return norm_chunks<T, W, 1>(px, x.ld, pr, r.ld, pw, eps, rows, cols, ph, ldh, out, stream);
-  if (cols <= 1024 * kVec * 2)
-    return norm_chunks<T, W, 2>(px, x.ld, pr, r.ld, pw, eps, rows, cols, ph, ldh, out, stream);
-  return norm_chunks<T, W, 4>(px, x.ld, pr, r.ld, pw, eps, rows, cols, ph, ldh, out, stream);
+cudaError_t norm_typed(const NormCall& n) {
+  if (n.cols <= 512 * kVec) return norm_chunks<T, W, 1, 512>(n);
+  if (n.cols <= 1024 * kVec) return norm_chunks<T, W, 2, 512>(n);
+  return norm_chunks<T, W, 2, 1024>(n);
 }
 
 }  // namespace
@@ -391,11 +590,12 @@ cudaError_t fp8_rms_norm_launch(Fp8In x, Fp8In residual, int type, const void* w
                                 cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return cudaSuccess;
   if (cols > kFp8NormMaxCols || rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-#define LLVQ_NORM(T, W) norm_typed<T, W>(x, residual, weight, eps, rows, cols, hidden, ld_hidden, out, stream)
-  if (type == LLVQ_DT_F32) return LLVQ_NORM(float, float);
-  if (type == LLVQ_DT_F16) return weight_type == LLVQ_DT_F32 ? LLVQ_NORM(__half, float) : LLVQ_NORM(__half, __half);
-  return weight_type == LLVQ_DT_F32 ? LLVQ_NORM(__nv_bfloat16, float) : LLVQ_NORM(__nv_bfloat16, __nv_bfloat16);
-#undef LLVQ_NORM
+  const NormCall n{x, residual, weight, eps, rows, cols, hidden, ld_hidden, out, stream};
+  if (type == LLVQ_DT_F32) return norm_typed<float, float>(n);
+  if (type == LLVQ_DT_F16)
+    return weight_type == LLVQ_DT_F32 ? norm_typed<__half, float>(n) : norm_typed<__half, __half>(n);
+  return weight_type == LLVQ_DT_F32 ? norm_typed<__nv_bfloat16, float>(n)
+                                    : norm_typed<__nv_bfloat16, __nv_bfloat16>(n);
 }
 
 }  // namespace llvq

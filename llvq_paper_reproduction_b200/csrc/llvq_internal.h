@@ -166,8 +166,8 @@ cudaError_t hadamard_launch(const void* in, int in_type, void* out, int out_type
 constexpr int kFp8Block = 128;
 constexpr int64_t kFp8NormMaxCols = 32768;  // a row of the norm stays in the registers of one CTA
 
-// Where a quantizer writes: e4m3 rows (row stride ld, a multiple of 8, base
-// 8-byte aligned) and the scale of row (or row block) r and column block b at
+// Where a quantizer writes: e4m3 rows (row stride ld, a multiple of 16, base
+// 16-byte aligned) and the scale of row (or row block) r and column block b at
 // scale[r * scale_row + b * scale_col].
 struct Fp8Out {
   uint8_t* q;

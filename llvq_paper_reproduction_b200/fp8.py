@@ -29,13 +29,18 @@ NORM_MAX_COLS = 32768
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # LLVQ_DT_*
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream().cuda_stream without building a Stream (3 us)
+_empty = torch.empty_strided  # the shortest way to a tensor of given strides
+
+
 def _launch(fn, device: torch.device, *args) -> None:
     """fn(*args, stream) on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            fn(*args, torch.cuda.current_stream().cuda_stream)
+            fn(*args, _raw_stream(index))
 
 
 def _input(x: torch.Tensor, name: str) -> torch.Tensor:
@@ -61,17 +66,16 @@ def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
-def _empty_e4m3(rows: int, cols: int, device: torch.device) -> torch.Tensor:
-    """Rows that start on 16-byte boundaries, as the product reads them."""
-    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=E4M3, device=device)
-    return q if cols % 16 == 0 else q[:, :cols]
+def _empty_e4m3(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    """Rows that start on 16-byte boundaries, as the product reads them, and their stride."""
+    ld = (cols + 15) // 16 * 16
+    return _empty((rows, cols), (ld, 1), dtype=E4M3, device=device), ld
 
 
-def _empty_rows(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+def _empty_rows(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, int, torch.Tensor]:
     """8-bit activations; their scales lie block by block (row fastest), as the product's warps read them."""
-    b = _blocks(cols)
-    return _empty_e4m3(rows, cols, device), torch.empty_strided((rows, b), (1, max(rows, 1)), dtype=torch.float32,
-                                                                device=device)
+    q, ld = _empty_e4m3(rows, cols, device)
+    return q, ld, _empty((rows, _blocks(cols)), (1, rows), dtype=torch.float32, device=device)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -81,9 +85,10 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     an infinity makes the block's scale infinite."""
     x = _input(x, "x")
     m, k = x.shape
-    q, scale = _empty_rows(m, k, x.device)
-    _launch(_native.fp8_quantize, x.device, x.data_ptr(), _TYPES[x.dtype], x.stride(0), m, k, 1, q.data_ptr(),
-            q.stride(0), scale.data_ptr(), 1, m)
+    device = x.device
+    q, ldq, scale = _empty_rows(m, k, device)
+    _launch(_native.fp8_quantize, device, x.data_ptr(), _TYPES[x.dtype], x.stride(0), m, k, 1, q.data_ptr(), ldq,
+            scale.data_ptr(), 1, m)
     return q, scale
 
 
@@ -92,10 +97,11 @@ def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``quantize_rows``, with one scale per 128 x 128 block (weights, laid out once)."""
     w = _input(w, "w")
     n, k = w.shape
-    q = _empty_e4m3(n, k, w.device)
-    scale = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
-    _launch(_native.fp8_quantize, w.device, w.data_ptr(), _TYPES[w.dtype], w.stride(0), n, k, BLOCK, q.data_ptr(),
-            q.stride(0), scale.data_ptr(), scale.stride(0), 1)
+    device, kb = w.device, _blocks(k)
+    q, ldq = _empty_e4m3(n, k, device)
+    scale = _empty((_blocks(n), kb), (kb, 1), dtype=torch.float32, device=device)
+    _launch(_native.fp8_quantize, device, w.data_ptr(), _TYPES[w.dtype], w.stride(0), n, k, BLOCK, q.data_ptr(), ldq,
+            scale.data_ptr(), kb, 1)
     return q, scale
 
 
@@ -106,9 +112,10 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Te
     gate, up = _input(gate, "gate"), _input(up, "up")
     _same(up, gate, "up")
     m, k = gate.shape
-    q, scale = _empty_rows(m, k, gate.device)
-    _launch(_native.fp8_swiglu, gate.device, gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0),
-            _TYPES[gate.dtype], m, k, q.data_ptr(), q.stride(0), scale.data_ptr(), 1, m)
+    device = gate.device
+    q, ldq, scale = _empty_rows(m, k, device)
+    _launch(_native.fp8_swiglu, device, gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0),
+            _TYPES[gate.dtype], m, k, q.data_ptr(), ldq, scale.data_ptr(), 1, m)
     return q, scale
 
 
@@ -120,24 +127,27 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
     x's type or fp32; at most 32,768 columns."""
     x = _input(x, "x")
     m, k = x.shape
-    if weight.shape != (k,) or weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"weight must be [{k}] of {x.dtype} or float32 on {x.device}")
+    device, dtype = x.device, x.dtype
+    if weight.shape != (k,) or weight.device != device or weight.dtype not in (dtype, torch.float32):
+        raise ValueError(f"weight must be [{k}] of {dtype} or float32 on {device}")
     if weight.requires_grad and torch.is_grad_enabled():
         raise ValueError("weight requires grad: the 8-bit operators are forward only (use torch.no_grad)")
     if k > NORM_MAX_COLS:
         raise ValueError(f"rms_norm takes at most {NORM_MAX_COLS} columns, got {k}")
-    weight = weight.contiguous()
-    q, scale = _empty_rows(m, k, x.device)
-    hidden = None
-    if residual is not None:
-        residual = _input(residual, "residual")
-        _same(residual, x, "residual")
-        hidden = torch.empty((m, k), dtype=x.dtype, device=x.device)
-    _launch(_native.fp8_rms_norm, x.device, x.data_ptr(), x.stride(0),
-            0 if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
-            _TYPES[x.dtype], weight.data_ptr(), _TYPES[weight.dtype], eps, m, k,
-            0 if hidden is None else hidden.data_ptr(), k, q.data_ptr(), q.stride(0), scale.data_ptr(), 1, m)
-    return (q, scale) if hidden is None else (q, scale, hidden)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    q, ldq, scale = _empty_rows(m, k, device)
+    args = (_TYPES[dtype], weight.data_ptr(), _TYPES[weight.dtype], eps, m, k)
+    if residual is None:
+        _launch(_native.fp8_rms_norm, device, x.data_ptr(), x.stride(0), 0, 0, *args, 0, k, q.data_ptr(), ldq,
+                scale.data_ptr(), 1, m)
+        return q, scale
+    residual = _input(residual, "residual")
+    _same(residual, x, "residual")
+    hidden = _empty((m, k), (k, 1), dtype=dtype, device=device)
+    _launch(_native.fp8_rms_norm, device, x.data_ptr(), x.stride(0), residual.data_ptr(), residual.stride(0), *args,
+            hidden.data_ptr(), k, q.data_ptr(), ldq, scale.data_ptr(), 1, m)
+    return q, scale, hidden
 
 
 def _operand(q: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
@@ -151,9 +161,18 @@ def _operand(q: torch.Tensor, name: str) -> tuple[torch.Tensor, int]:
             return q, (cols + 15) // 16 * 16
         if q.stride(0) % 16 == 0 and q.stride(0) >= cols:
             return q, q.stride(0)
-    copy = _empty_e4m3(rows, cols, q.device)
+    copy, ld = _empty_e4m3(rows, cols, q.device)
     copy.view(torch.uint8).copy_(q.view(torch.uint8))
-    return copy, (cols + 15) // 16 * 16
+    return copy, ld
+
+
+def _scales(s: torch.Tensor, rows: int, blocks: int, device: torch.device, name: str) -> tuple[int, int, int]:
+    if s.dtype != torch.float32 or s.shape != (rows, blocks) or s.device != device:
+        raise ValueError(f"{name} must be float32 [{rows}, {blocks}] on {device}, got {s.dtype} {tuple(s.shape)} on "
+                         f"{s.device}")
+    if s.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: the 8-bit operators are forward only (use torch.no_grad)")
+    return s.data_ptr(), *s.stride()
 
 
 def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -173,18 +192,14 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     (m, k), (n, kw) = a.shape, w.shape
     if k != kw:
         raise ValueError(f"a has {k} columns, w has {kw}")
-    for s, rows, name in ((a_scale, m, "a_scale"), (w_scale, _blocks(n), "w_scale")):
-        if s.dtype != torch.float32 or s.shape != (rows, _blocks(k)):
-            raise ValueError(f"{name} must be float32 [{rows}, {_blocks(k)}], got {s.dtype} {tuple(s.shape)}")
-        if s.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires grad: the 8-bit operators are forward only (use torch.no_grad)")
-    device = a.device
-    if w.device != device or a_scale.device != device or w_scale.device != device:
-        raise ValueError("a, w and their scales must be on one device")
-    y = torch.empty((m, n), dtype=out_dtype, device=device)
-    _launch(_native.fp8_gemm, device, a.data_ptr(), lda, a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1),
-            w.data_ptr(), ldw, w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1), m, n, k, y.data_ptr(), n,
-            _TYPES[out_dtype], _flag(device).data_ptr())
+    device, kb = a.device, _blocks(k)
+    if w.device != device:
+        raise ValueError(f"a is on {device}, w on {w.device}")
+    a_s, w_s = _scales(a_scale, m, kb, device, "a_scale"), _scales(w_scale, _blocks(n), kb, device, "w_scale")
+    y = _empty((m, n), (n, 1), dtype=out_dtype, device=device)
+    flag = _flags.get(device.index)
+    _launch(_native.fp8_gemm, device, a.data_ptr(), lda, *a_s, w.data_ptr(), ldw, *w_s, m, n, k, y.data_ptr(), n,
+            _TYPES[out_dtype], (_flag(device) if flag is None else flag).data_ptr())
     if check:
         raise_pending_errors(device)
     return y
@@ -195,13 +210,10 @@ _flags: dict[int, torch.Tensor] = {}
 
 
 def _flag(device: torch.device) -> torch.Tensor:
-    f = _flags.get(device.index)
-    if f is None:
-        if torch.cuda.is_current_stream_capturing():
-            # memory taken during a capture belongs to that graph
-            raise RuntimeError("call fp8.gemm once on this device before capturing it in a CUDA graph")
-        f = _flags.setdefault(device.index, torch.zeros((1,), dtype=torch.int32, device=device))
-    return f
+    if torch.cuda.is_current_stream_capturing():
+        # memory taken during a capture belongs to that graph
+        raise RuntimeError("call fp8.gemm once on this device before capturing it in a CUDA graph")
+    return _flags.setdefault(device.index, torch.zeros((1,), dtype=torch.int32, device=device))
 
 
 def pending_errors(device: str | torch.device = "cuda") -> dict:
