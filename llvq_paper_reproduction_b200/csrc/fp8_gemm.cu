@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <cstring>
 #include <type_traits>
 
 #include "llvq_b200.h"
@@ -30,11 +31,19 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // gemm.cu
 namespace {
 
 constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr int kMaxSplits = 8;  // CTAs that share a tile's K blocks: a portable cluster
+
+template <typename T>
+__device__ __forceinline__ T to_out(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
 
 __device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type) {
   if (type == LLVQ_DT_F32) static_cast<float*>(y)[i] = v;
-  else if (type == LLVQ_DT_F16) static_cast<__half*>(y)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+  else if (type == LLVQ_DT_F16) static_cast<__half*>(y)[i] = to_out<__half>(v);
+  else static_cast<__nv_bfloat16*>(y)[i] = to_out<__nv_bfloat16>(v);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -45,26 +54,28 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type)
 // memory in rank order.
 //
 // Roles: warp 0 loads both operands with TMA, warp 1 issues the MMAs, warps
-// 2..5 add up.  TMEM holds kBufs block sums so the MMAs run ahead of the
-// additions.  The scales of a block (kAct row scales and the tile's weight
-// scale) travel through a ring of kRing slots filled with cp.async.
+// 2..5 add up.  The adders take kGroup blocks at a time (64 columns of TMEM, one
+// load): a pass is a chain of latencies, about 1000 cycles however narrow the
+// sums are.  TMEM holds kBufs such groups so the MMAs run ahead.  Scales come
+// with cp.async, kChunk blocks at a time and one chunk ahead.
 constexpr int kFewThreads = 192;
 constexpr int kTileRows = 128;
-constexpr int kRing = 8;
 
 template <int kAct>
 struct Few {
   static constexpr int kStageBytes = kTileRows * 128 + kAct * 128;
   // two CTAs per SM: at least 76 KB each, so that a third, which could run out of TMEM, never fits
-  static constexpr int kStages = (100 * 1024) / kStageBytes;
-  static constexpr int kTmemCols = kAct <= 16 ? 128 : 256;
-  static constexpr int kBufs = kTmemCols / kAct > 8 ? 8 : kTmemCols / kAct;
-  static constexpr int kRingFloats = kAct + 4;  // row scales, then the weight scale
-  static constexpr int kRingOff = kStages * kStageBytes;
-  static constexpr int kBarOff = kRingOff + kRing * kRingFloats * 4;
+  static constexpr int kStages = (98 * 1024) / kStageBytes;
+  static constexpr int kGroup = kAct < 64 ? 64 / kAct : 1;
+  static constexpr int kTmemCols = 256;
+  static constexpr int kBufs = kTmemCols / (kAct * kGroup);
+  static constexpr int kChunk = 1024 / kAct < 64 ? 1024 / kAct : 64;  // blocks
+  static constexpr int kScaleFloats = kChunk * (kAct + 4);  // row scales of every block, then its weight scale
+  static constexpr int kScaleOff = kStages * kStageBytes;
+  static constexpr int kBarOff = kScaleOff + 2 * kScaleFloats * 4;
   static constexpr int kBars = 2 * kStages + 2 * kBufs + 1;
   static constexpr size_t kSmem = (size_t)kBarOff + 8 * kBars + 16 + 1024;
-  static_assert(kStages >= 3 && kAct * kTileRows * 4 <= kRingOff && kRingOff % 16 == 0 && kBarOff % 8 == 0);
+  static_assert(kStages >= 2 && kAct * kTileRows * 4 <= kScaleOff && kScaleOff % 16 == 0 && kBarOff % 8 == 0);
   static_assert(kSmem > 76 * 1024 && kSmem <= 113 * 1024);
 };
 
@@ -80,7 +91,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + F::kBarOff);
   uint32_t* holder = reinterpret_cast<uint32_t*>(bars + F::kBars);
-  float* ring = reinterpret_cast<float*>(base + F::kRingOff);
   const uint32_t sbase = tc::smem_addr(base);
   auto full = [&](int st) { return tc::smem_addr(&bars[st]); };
   auto empty = [&](int st) { return tc::smem_addr(&bars[F::kStages + st]); };
@@ -92,6 +102,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int n0 = tile * kTileRows, m0 = (int)blockIdx.y * kAct;
   const int b_begin = (int)((int64_t)blocks * rank / splits), b_end = (int)((int64_t)blocks * (rank + 1) / splits);
   const int count = b_end - b_begin;
+  auto load_stage = [&](int i) {
+    const int st = i % F::kStages;
+    const uint32_t dst = sbase + st * F::kStageBytes;
+    tc::mbar_arrive_expect_tx(full(st), F::kStageBytes);
+    tc::tma_load_2d(dst, &tw, (b_begin + i) * kFp8Block, n0, full(st));
+    tc::tma_load_2d(dst + kTileRows * 128, &ta, (b_begin + i) * kFp8Block, m0, full(st));
+  };
   if (tid == 0) {
     for (int i = 0; i < F::kStages; ++i) {
       tc::mbar_init(full(i), 1);
@@ -103,8 +120,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     }
     tc::mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+    // the first loads are under way while the CTA sets up
+    for (int i = 0; i < F::kStages && i < count; ++i) load_stage(i);
   }
-  if (warp == 0) tc::tmem_alloc(tc::smem_addr(holder), F::kTmemCols);
+  if (warp == 1) tc::tmem_alloc(tc::smem_addr(holder), F::kTmemCols);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -114,82 +134,100 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 
   if (warp == 0) {
     if (lane == 0) {  // TMA producer
-      int i = 0;
+      int i = F::kStages;
       for (; i < count; ++i) {
-        const int st = i % F::kStages, use = i / F::kStages;
-        if (use > 0 && !tc::mbar_wait(empty(st), (use - 1) & 1, kWaitLimit)) {
+        if (!tc::mbar_wait(empty(i % F::kStages), (i / F::kStages - 1) & 1, kWaitLimit)) {
           failed = true;
           break;
         }
-        const uint32_t dst = sbase + st * F::kStageBytes;
-        tc::mbar_arrive_expect_tx(full(st), F::kStageBytes);
-        tc::tma_load_2d(dst, &tw, (b_begin + i) * kFp8Block, n0, full(st));
-        tc::tma_load_2d(dst + kTileRows * 128, &ta, (b_begin + i) * kFp8Block, m0, full(st));
+        load_stage(i);
       }
       // no copy may still be in flight when the block exits: wait for the last use of every stage
+      i = min(i, count);
       for (int u = i > F::kStages ? i - F::kStages : 0; u < i; ++u)
         tc::mbar_wait(full(u % F::kStages), (u / F::kStages) & 1, kWaitLimit);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {  // MMA issuer
-      constexpr uint32_t idesc = tc::idesc_e4m3_f32(kTileRows, kAct);
-      for (int i = 0; i < count; ++i) {
-        const int st = i % F::kStages, buf = i % F::kBufs, use = i / F::kBufs;
-        if ((use > 0 && !tc::mbar_wait(acc_empty(buf), (use - 1) & 1, kWaitLimit)) ||
-            !tc::mbar_wait(full(st), (i / F::kStages) & 1, kWaitLimit)) {
-          failed = true;
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t sw = sbase + st * F::kStageBytes, sa = sw + kTileRows * 128;
+  } else if (warp == 1) {  // MMA issuer: the warp waits, one thread issues
+    constexpr uint32_t idesc = tc::idesc_e4m3_f32(kTileRows, kAct);
+    const bool issuer = tc::elect_one();
+    const uint64_t desc0 = tc::desc_sw128(sbase);
+    uint32_t st = 0, st_use = 0;
+    for (int i = 0; i < count; ++i) {
+      const uint32_t in_group = i % F::kGroup, buf = i / F::kGroup % F::kBufs, use = i / F::kGroup / F::kBufs;
+      if ((in_group == 0 && use > 0 && !tc::mbar_wait(acc_empty(buf), (use - 1) & 1u, kWaitLimit)) ||
+          !tc::mbar_wait(full(st), st_use & 1u, kWaitLimit)) {
+        failed = true;
+        break;
+      }
+      tc::fence_after_sync();
+      if (issuer) {
+        const uint64_t dw = desc0 + st * (F::kStageBytes >> 4), da = dw + (kTileRows * 128 >> 4);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          tc::mma_f8(tmem + buf * kAct, tc::desc_sw128(sw + ks * 32), tc::desc_sw128(sa + ks * 32), idesc, ks > 0);
+          tc::mma_f8(tmem + (buf * F::kGroup + in_group) * kAct, dw + 2 * ks, da + 2 * ks, idesc, ks > 0);
         tc::commit(empty(st));
-        tc::commit(acc_full(buf));
+        if (in_group == F::kGroup - 1 || i == count - 1) tc::commit(acc_full(buf));
       }
-      // every MMA issued has finished before TMEM is freed
-      tc::commit(drain);
-      tc::mbar_wait(drain, 0, kWaitLimit);
+      __syncwarp();
+      if (++st == F::kStages) st = 0, ++st_use;
     }
+    // every MMA issued has finished before TMEM is freed
+    if (issuer) tc::commit(drain);
+    __syncwarp();
+    tc::mbar_wait(drain, 0, kWaitLimit);
   } else {  // warps 2..5 read TMEM lane quarters 2, 3, 0, 1
     const int t = tid - 64;
     const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    // scales of block i into slot i % kRing: thread t brings row scale t, thread 0 the weight scale too
-    auto fetch = [&](int i) {
-      if (i < count) {
-        float* slot = ring + (i % kRing) * F::kRingFloats;
-        const int64_t b = b_begin + i;
-        if (t < kAct) {
-          const bool live = m0 + t < m_total;
-          tc::cp_async4(tc::smem_addr(slot + t), as + (live ? (m0 + t) * as_row + b * as_col : 0), live);
-        }
-        if (t == 0) tc::cp_async4(tc::smem_addr(slot + kAct), ws + tile * ws_row + b * ws_col, true);
+    float* scales = reinterpret_cast<float*>(base + F::kScaleOff);
+    // chunk c of kChunk blocks into half c & 1 of the scales
+    auto fetch = [&](int c) {
+      const int first = c * F::kChunk, last = min(count, first + F::kChunk);
+      const uint32_t half = tc::smem_addr(scales + (c & 1) * F::kScaleFloats);
+      for (int e = t; e < (last - first) * kAct; e += 128) {
+        const int i = e / kAct, j = e % kAct;
+        const bool live = m0 + j < m_total;
+        tc::cp_async4(half + (i * (kAct + 4) + j) * 4,
+                      as + (live ? (m0 + j) * as_row + (b_begin + first + i) * as_col : 0), live);
       }
+      for (int i = t; i < last - first; i += 128)
+        tc::cp_async4(half + (i * (kAct + 4) + kAct) * 4, ws + tile * ws_row + (b_begin + first + i) * ws_col, true);
       tc::cp_async_commit();
     };
 #pragma unroll
     for (int j = 0; j < kAct; ++j) acc[j] = 0.f;
-    for (int i = 0; i < kRing - 1; ++i) fetch(i);
-    for (int i = 0; i < count; ++i) {
-      const int buf = i % F::kBufs;
-      tc::cp_async_wait<kRing - 2>();
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // slot i is whole, and nobody reads slot i - 1 any more
-      fetch(i + kRing - 1);
-      if (!failed && !tc::mbar_wait(acc_full(buf), (i / F::kBufs) & 1, kWaitLimit)) failed = true;
-      tc::fence_after_sync();
-      const float* slot = ring + (i % kRing) * F::kRingFloats;
-      const float wsc = slot[kAct];
-#pragma unroll
-      for (int c = 0; c < kAct; c += 16) {
-        float v[16];
-        tc::tmem_ld16(t0 + buf * kAct + c, v);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(v[j] * wsc, slot[c + j], acc[c + j]);
+    fetch(0);
+    for (int i0 = 0; i0 < count; i0 += F::kGroup) {
+      if (i0 % F::kChunk == 0) {
+        tc::cp_async_wait<0>();
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // this chunk is whole, and nobody reads the last one any more
+        if (i0 + F::kChunk < count) fetch(i0 / F::kChunk + 1);
       }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(acc_empty(buf));
+      const int buf = i0 / F::kGroup % F::kBufs;
+      if (!failed && !tc::mbar_wait(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1, kWaitLimit)) failed = true;
+      tc::fence_after_sync();
+      const float* slot = scales + (i0 / F::kChunk & 1) * F::kScaleFloats + i0 % F::kChunk * (kAct + 4);
+#pragma unroll
+      for (int c = 0; c < F::kGroup * kAct; c += 32) {
+        uint32_t v[32];
+        tc::tmem_ld32(t0 + buf * (F::kGroup * kAct) + c, v);
+        tc::tmem_wait_ld();
+        if (c + 32 == F::kGroup * kAct) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(acc_empty(buf));
+        }
+#pragma unroll
+        for (int q = 0; q < 32; q += 16) {
+          const int u = (c + q) / kAct, j0 = (c + q) % kAct;
+          if (i0 + u < count) {
+            const float* row = slot + u * (kAct + 4);
+            const float w = row[kAct];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              acc[j0 + j] = fmaf(__uint_as_float(v[q + j]) * w, row[j0 + j], acc[j0 + j]);
+          }
+        }
+      }
     }
     const int n = n0 + (warp & 3) * 32 + lane;
     if (splits == 1) {
@@ -211,8 +249,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       const int t = tid - 64, n = n0 + t;
       for (int j = rank; j < kAct && m0 + j < m_total; j += splits) {
         const uint32_t at = sbase + (uint32_t)(j * kTileRows + t) * 4;
-        float sum = 0.f;
-        for (int r = 0; r < splits; ++r) sum += tc::ld_cluster(tc::map_rank(at, r));
+        float part[kMaxSplits], sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) part[r] = r < splits ? tc::ld_cluster(tc::map_rank(at, r)) : 0.f;
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) sum += part[r];  // the zeros past splits change nothing
         if (n < n_total) store_out(y, (int64_t)(m0 + j) * ldy + n, sum, y_type);
       }
     }
@@ -222,48 +263,53 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (warp == 0) tc::tmem_dealloc(tmem, F::kTmemCols);
+  if (warp == 1) tc::tmem_dealloc(tmem, F::kTmemCols);
 }
 
 // ---------------------------------------------------------------- many rows
-// Two CTAs of a cluster share a tile of 256 activation rows x kTileN weight
-// rows (tcgen05 cta_group::2, M = 256): each loads 128 activation rows and
-// half of the weight rows, so a CTA reads 16 + kTileN / 16 KB per block for
-// 128 x kTileN outputs, two thirds of what a CTA alone would at 256.  TMEM lane = activation row,
-// so a lane's scale for a block is one number, a_scale[row] w_scale, and the
-// addition is one packed fused multiply-add per two outputs.
+// Activations are the M side: TMEM lane = activation row, so a lane's scale
+// for a block is one number, a_scale[row] w_scale, and the addition is one
+// packed fused multiply-add per two outputs.  Tiles are 256 weight rows wide.
+//
+// Wide<2>: two CTAs of a cluster share a tile of 256 activation rows (tcgen05
+// cta_group::2, M = 256); each loads 128 activation rows and half of the weight
+// rows, so a block costs a CTA 32 KB for 128 x 256 outputs instead of 48.
+// Persistent: one pair per two SMs.
+// Wide<1>: a CTA per tile of 128 activation rows, where that fits one wave; the
+// K blocks are split over a cluster, which adds its partial sums through
+// distributed shared memory in rank order.
 //
 // Roles: warps 0..15 add up (lane quarter warp % 4, column quarter warp / 4),
-// warp 16 loads with TMA, warp 17 of the leading CTA issues the MMAs of both,
-// warps 18 and 19 bring the scales, kScaleGroup blocks at a time and two
-// groups in flight.  Adding is a chain of waits (block sum ready, TMEM load, hand
-// back), so it takes four warps per scheduler to keep up with the tensor
-// cores: with two, of twice the columns, a block took 1300 cycles for the 512
-// of its MMAs.  TMEM holds kBufs block sums of kTileN columns.  The leader's
-// full[] takes the bytes of both CTAs' loads; empty[] and acc_full[] are
-// committed in both CTAs; the leader's acc_empty[] takes the arrivals of all 32
-// adding warps.
+// warp 16 loads with TMA, warp 17 (of the leading CTA) issues the MMAs, warps
+// 18 and 19 bring the scales, kScaleGroup blocks at a time and two groups in
+// flight.  Adding is a chain of waits (block sum ready, TMEM load, hand back),
+// so it takes four warps per scheduler to keep up with the tensor cores: with
+// two, of twice the columns, a block took 1300 cycles for the 512 of its MMAs.
+// TMEM holds two block sums of 256 columns.  In a pair the leader's full[]
+// takes the bytes of both CTAs' loads; empty[] and acc_full[] are committed in
+// both CTAs; the leader's acc_empty[] takes the arrivals of all 32 adding warps.
 constexpr int kAddWarps = 16;
-constexpr int kPairThreads = kAddWarps * 32 + 128;
+constexpr int kWideThreads = kAddWarps * 32 + 128;
 // 640 threads launch with 96 registers each: 61,440 = 512 x 112 + 128 x 32
 constexpr int kAddRegs = 112, kOtherRegs = 32;
-constexpr int kPairRows = 256;
-constexpr int kScaleGroup = 8;
-constexpr int kScaleBlock = 2 * 128 * 8;  // bytes of a block's scales: 2 column halves x 128 rows x (pre, factor)
+constexpr int kTileN = 256;
+constexpr int kCols = kTileN / (kAddWarps / 4);  // columns of an adding warp
+constexpr int kAccBufs = 512 / kTileN;
+constexpr int kScaleGroup = 8, kScaleGroups = 2;
+constexpr int kScaleBlock = (128 + 4) * 4;  // bytes of a block's scales: 128 rows, two column halves
 
-template <int kTileN>
-struct Pair {
-  static constexpr int kStageA = 128 * 128, kStageB = kTileN / 2 * 128;
+template <int kCtas>
+struct Wide {
+  static constexpr int kStageA = 128 * 128, kStageB = kTileN / kCtas * 128;
   static constexpr int kStageBytes = kStageA + kStageB;
-  static constexpr int kStages = 128 * 1024 / kStageBytes;
-  static constexpr int kBufs = 512 / kTileN;
-  static constexpr int kCols = kTileN / (kAddWarps / 4);  // columns of an adding warp
-  static constexpr int kStoreOff = kStages * kStageBytes;      // 4 KB per adding warp
-  static constexpr int kScaleOff = kStoreOff + kAddWarps * 4096;
-  static constexpr int kBarOff = kScaleOff + 2 * kScaleGroup * kScaleBlock;
-  static constexpr int kBars = 2 * kStages + 2 * kBufs + 5;
+  static constexpr int kStages = 4;
+  // 4 KB per adding warp to store through; a CTA with a single tile stores when its stages are free
+  static constexpr int kStoreOff = kCtas == 2 ? kStages * kStageBytes : 0;
+  static constexpr int kScaleOff = kCtas == 2 ? kStoreOff + kAddWarps * 4096 : kStages * kStageBytes;
+  static constexpr int kBarOff = kScaleOff + kScaleGroups * kScaleGroup * kScaleBlock;
+  static constexpr int kBars = 2 * kStages + 2 * kAccBufs + 2 * kScaleGroups + 1;
   static constexpr size_t kSmem = (size_t)kBarOff + 8 * kBars + 16 + 1024;
-  static_assert(kSmem <= 227 * 1024);
+  static_assert(kSmem <= 227 * 1024 && kScaleOff >= 128 * kTileN * 4);
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
@@ -305,16 +351,22 @@ __device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, float pre
   for (int j = 0; j < kCount / 2; ++j) acc[j] = fma2(pack2(v[2 * j], v[2 * j + 1]), ff, acc[j]);
 }
 
-// A warp's 32 rows x kCols columns to y, through its 4 KB of shared memory (32
+// y as rows of 16-byte chunks where its base and stride allow.
+template <typename T>
+__device__ __forceinline__ bool whole_chunks(const T* y, int64_t ldy) {
+  return ldy * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+}
+
+// A warp's 32 rows x kWidth columns to y, through its 4 KB of shared memory (32
 // rows of 128 bytes, 16-byte chunks swizzled by the row) so that the global
 // stores are whole 128-byte lines.
-template <typename T, int kCols>
+template <typename T, int kWidth>
 __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0,
                                            int col0, int m_total, int n_total, int lane) {
   constexpr int kPerLine = 128 / (int)sizeof(T), kPerChunk = 16 / (int)sizeof(T);
-  const bool whole = ldy * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  const bool whole = whole_chunks(y, ldy);
 #pragma unroll
-  for (int c0 = 0; c0 < kCols; c0 += kPerLine) {
+  for (int c0 = 0; c0 < kWidth; c0 += kPerLine) {
 #pragma unroll
     for (int ch = 0; ch < 8; ++ch) {
       alignas(16) T e[kPerChunk];
@@ -322,16 +374,8 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T*
       for (int j = 0; j < kPerChunk; j += 2) {
         float lo, hi;
         unpack2(acc[(c0 + ch * kPerChunk + j) / 2], lo, hi);
-        if constexpr (sizeof(T) == 4) {
-          e[j] = lo;
-          e[j + 1] = hi;
-        } else if constexpr (std::is_same_v<T, __half>) {
-          e[j] = __float2half_rn(lo);
-          e[j + 1] = __float2half_rn(hi);
-        } else {
-          e[j] = __float2bfloat16_rn(lo);
-          e[j + 1] = __float2bfloat16_rn(hi);
-        }
+        e[j] = to_out<T>(lo);
+        e[j + 1] = to_out<T>(hi);
       }
       *reinterpret_cast<uint4*>(buf + lane * 128 + ((ch ^ (lane & 7)) * 16)) = *reinterpret_cast<const uint4*>(e);
     }
@@ -366,13 +410,58 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& mt, int& nt)
   nt = in / height;
 }
 
-template <int kTileN>
-__global__ void __launch_bounds__(kPairThreads, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tw, int blocks,
+// Partial sums of a tile in shared memory: rows of 256 fp32, 16-byte chunks swizzled by the row.
+__device__ __forceinline__ uint32_t partial_at(uint32_t base, int row, int chunk) {
+  return base + (uint32_t)row * (kTileN * 4) + (uint32_t)((chunk ^ (row & 7)) * 16);
+}
+
+// This CTA's rows (a 1 / splits share) of the tile, added over the cluster in rank order.
+template <typename T>
+__device__ __forceinline__ void store_reduced(uint32_t partial, int rank, int splits, T* __restrict__ y, int64_t ldy,
+                                              int m0, int n0, int m_total, int n_total, int warp, int lane) {
+  const bool whole = whole_chunks(y, ldy);
+  const int end = min((rank + 1) * 128 / splits, m_total - m0);
+  for (int r = rank * 128 / splits + warp; r < end; r += kAddWarps) {
+#pragma unroll
+    for (int c = 0; c < kTileN / 128; ++c) {
+      const int chunk = c * 32 + lane, col = n0 + chunk * 4;
+      if (col >= n_total) continue;
+      float4 part[kMaxSplits], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s)  // all the reads under way before the first sum
+        part[s] = s < splits ? tc::ld_cluster4(tc::map_rank(partial_at(partial, r, chunk), s))
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kMaxSplits; ++s)
+        sum.x += part[s].x, sum.y += part[s].y, sum.z += part[s].z, sum.w += part[s].w;
+      T e[4] = {to_out<T>(sum.x), to_out<T>(sum.y), to_out<T>(sum.z), to_out<T>(sum.w)};
+      T* dst = y + (int64_t)(m0 + r) * ldy + col;
+      if (whole && col + 4 <= n_total) {
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<float4*>(dst) = make_float4(e[0], e[1], e[2], e[3]);
+        } else {
+          uint2 w;
+          memcpy(&w, e, 8);
+          *reinterpret_cast<uint2*>(dst) = w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < n_total) dst[j] = e[j];
+      }
+    }
+  }
+}
+
+// Wide<2>: `split` is 1 and a pair takes tiles pair, + pairs, ...  Wide<1>: one
+// tile per cluster of `split` CTAs.
+template <int kCtas>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tw, int blocks_total,
                 const float* __restrict__ as, int64_t as_row, int64_t as_col, const float* __restrict__ ws,
                 int64_t ws_row, int64_t ws_col, int m_total, int n_total, void* __restrict__ y, int64_t ldy, int y_type,
-                int tm, int tn, int* error_flag) {
-  using P = Pair<kTileN>;
+                int tm, int tn, int splits, int* error_flag) {
+  using P = Wide<kCtas>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -382,45 +471,62 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   auto full = [&](int st) { return tc::smem_addr(&bars[st]); };
   auto empty = [&](int st) { return tc::smem_addr(&bars[P::kStages + st]); };
   auto acc_full = [&](int b) { return tc::smem_addr(&bars[2 * P::kStages + b]); };
-  auto acc_empty = [&](int b) { return tc::smem_addr(&bars[2 * P::kStages + P::kBufs + b]); };
-  auto scale_full = [&](int i) { return tc::smem_addr(&bars[2 * P::kStages + 2 * P::kBufs + i]); };
-  auto scale_empty = [&](int i) { return tc::smem_addr(&bars[2 * P::kStages + 2 * P::kBufs + 2 + i]); };
+  auto acc_empty = [&](int b) { return tc::smem_addr(&bars[2 * P::kStages + kAccBufs + b]); };
+  auto scale_full = [&](int i) { return tc::smem_addr(&bars[2 * P::kStages + 2 * kAccBufs + i]); };
+  auto scale_empty = [&](int i) { return tc::smem_addr(&bars[2 * P::kStages + 2 * kAccBufs + kScaleGroups + i]); };
   const uint32_t drain = tc::smem_addr(&bars[P::kBars - 1]);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)tc::cluster_rank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
-  const int tiles = tm * tn;
-  if (tid == 0) {
+  // rank: of the CTA in its pair; part: its share of the K blocks
+  const int rank = kCtas == 2 ? (int)tc::cluster_rank() : 0, part = kCtas == 1 ? (int)tc::cluster_rank() : 0;
+  const int tiles = tm * tn, first = kCtas == 2 ? (int)blockIdx.x >> 1 : (int)blockIdx.x / splits;
+  const int step = kCtas == 2 ? (int)gridDim.x >> 1 : tiles;
+  const int b_begin = (int)((int64_t)blocks_total * part / splits);
+  const int blocks = (int)((int64_t)blocks_total * (part + 1) / splits) - b_begin;
+  auto load_stage = [&](uint32_t st, int b, int m0, int n0) {
+    const uint32_t dst = sbase + st * P::kStageBytes, bar = kCtas == 2 ? tc::map_rank(full(st), 0) : full(st);
+    if (rank == 0) tc::mbar_arrive_expect_tx(full(st), kCtas * P::kStageBytes);
+    tc::Ctas<kCtas>::tma_load(dst, &ta, (b_begin + b) * kFp8Block, m0, bar);
+    tc::Ctas<kCtas>::tma_load(dst + P::kStageA, &tw, (b_begin + b) * kFp8Block, n0, bar);
+  };
+  if (tid == kAddWarps * 32) {  // the producer
     for (int i = 0; i < P::kStages; ++i) {
       tc::mbar_init(full(i), 1);
       tc::mbar_init(empty(i), 1);
     }
-    for (int i = 0; i < P::kBufs; ++i) {
+    for (int i = 0; i < kAccBufs; ++i) {
       tc::mbar_init(acc_full(i), 1);
-      tc::mbar_init(acc_empty(i), 2 * kAddWarps);
+      tc::mbar_init(acc_empty(i), kCtas * kAddWarps);
     }
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(scale_full(i), 2);
+    for (int i = 0; i < kScaleGroups; ++i) {
+      tc::mbar_init(scale_full(i), 64);  // the threads of two warps, when their copies are there
       tc::mbar_init(scale_empty(i), kAddWarps);
     }
     tc::mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+    if (kCtas == 1) {  // nothing to wait for: the first loads are under way while the CTA sets up
+      int mt, nt;
+      tile_at(first, tm, tn, mt, nt);
+      for (int b = 0; b < P::kStages && b < blocks; ++b) load_stage(b, b, mt * 128, nt * kTileN);
+    }
   }
   __syncwarp();
-  if (warp == kAddWarps) tc::tmem_alloc_pair(tc::smem_addr(holder), 512);
+  if (warp == kAddWarps + 1) tc::Ctas<kCtas>::alloc(tc::smem_addr(holder), 512);
   tc::fence_before_sync();
-  tc::cluster_sync();
+  if (kCtas == 1) __syncthreads();
+  else tc::cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *holder;
   bool failed = false;
 
   if (warp >= kAddWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == kAddWarps && lane == 0) {  // TMA producer of this CTA's halves
+    if (warp == kAddWarps && lane == 0) {  // TMA producer of this CTA's operands
       uint32_t g = 0;
-      for (int t = pair; t < tiles && !failed; t += pairs) {
+      for (int t = first; t < tiles && !failed; t += step) {
         int mt, nt;
         tile_at(t, tm, tn, mt, nt);
-        const int m0 = mt * kPairRows + rank * 128, n0 = nt * kTileN + rank * (kTileN / 2);
+        const int m0 = (mt * kCtas + rank) * 128, n0 = nt * kTileN + rank * (kTileN / kCtas);
         for (int b = 0; b < blocks; ++b, ++g) {
           const int st = (int)(g % P::kStages);
           const uint32_t use = g / P::kStages;
@@ -428,22 +534,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             failed = true;
             break;
           }
-          const uint32_t dst = sbase + st * P::kStageBytes, bar = tc::map_rank(full(st), 0);
-          if (rank == 0) tc::mbar_arrive_expect_tx(full(st), 2 * P::kStageBytes);
-          tc::tma_load_2d_pair(dst, &ta, b * kFp8Block, m0, bar);
-          tc::tma_load_2d_pair(dst + P::kStageA, &tw, b * kFp8Block, n0, bar);
+          if (kCtas == 2 || use > 0) load_stage(st, b, m0, n0);
         }
       }
       // every stage loaded has been consumed before the CTA may exit
       for (uint32_t u = g > (uint32_t)P::kStages ? g - P::kStages : 0u; u < g; ++u)
         if (!tc::mbar_wait(empty((int)(u % P::kStages)), (u / P::kStages) & 1u, kWaitLimit)) failed = true;
     }
-    if (warp == kAddWarps + 1 && rank == 0) {  // MMA issuer of the pair: the warp waits, one thread issues
-      constexpr uint32_t idesc = tc::idesc_e4m3_f32(kPairRows, kTileN);
+    if (warp == kAddWarps + 1 && rank == 0) {  // MMA issuer: the warp waits, one thread issues
+      constexpr uint32_t idesc = tc::idesc_e4m3_f32(128 * kCtas, kTileN);
       const bool issuer = tc::elect_one();
       const uint64_t desc0 = tc::desc_sw128(sbase);
       uint32_t st = 0, st_use = 0, buf = 0, buf_use = 0;
-      for (int t = pair; t < tiles && !failed; t += pairs) {
+      for (int t = first; t < tiles && !failed; t += step) {
         for (int b = 0; b < blocks; ++b) {
           // even lanes poll for the operands, odd ones for the TMEM columns: one latency instead of two
           const uint32_t bar = (lane & 1) ? acc_empty(buf) : full(st);
@@ -457,121 +560,135 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (issuer) {
             const uint64_t da = desc0 + st * (P::kStageBytes >> 4), dw = da + (P::kStageA >> 4);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) tc::mma_f8_pair(tmem + buf * kTileN, da + 2 * ks, dw + 2 * ks, idesc, ks > 0);
-            tc::commit_pair(acc_full(buf));
-            tc::commit_pair(empty(st));
+            for (int ks = 0; ks < 4; ++ks)
+              tc::Ctas<kCtas>::mma(tmem + buf * kTileN, da + 2 * ks, dw + 2 * ks, idesc, ks > 0);
+            tc::Ctas<kCtas>::commit(acc_full(buf));
+            tc::Ctas<kCtas>::commit(empty(st));
           }
           __syncwarp();
           if (++st == P::kStages) st = 0, ++st_use;
-          if (++buf == P::kBufs) buf = 0, ++buf_use;
+          if (++buf == kAccBufs) buf = 0, ++buf_use;
         }
       }
       // every MMA issued has finished before TMEM is freed
-      if (issuer) tc::commit_pair(drain);
+      if (issuer) tc::Ctas<kCtas>::commit(drain);
       __syncwarp();
       tc::mbar_wait(drain, 0, kWaitLimit);
     }
-    if (warp >= kAddWarps + 2) {  // scales: thread i brings those of rows i and i + 64 for both column halves
+    if (warp >= kAddWarps + 2) {  // scales: thread i copies those of rows i and i + 64, threads 0 and 1 the weights'
       const int i = tid - (kAddWarps + 2) * 32;
-      uint32_t gg = 0;
-      for (int t = pair; t < tiles && !failed; t += pairs) {
+      uint32_t slot = 0, use = 0;
+      for (int t = first; t < tiles && !failed; t += step) {
         int mt, nt;
         tile_at(t, tm, tn, mt, nt);
-        const int row0 = mt * kPairRows + rank * 128 + i, block0 = nt * kTileN / kFp8Block;
-        const int block1 = block0 + (kTileN > kFp8Block && nt * kTileN + kFp8Block < n_total ? 1 : 0);
-        const bool live0 = row0 < m_total, live1 = row0 + 64 < m_total;
+        const int row0 = (mt * kCtas + rank) * 128 + i, half = nt * (kTileN / kFp8Block) + i;
+        const bool live0 = row0 < m_total, live1 = row0 + 64 < m_total, live2 = half * kFp8Block < n_total;
         const float *pa0 = as + (live0 ? row0 * as_row : 0), *pa1 = as + (live1 ? (row0 + 64) * as_row : 0);
-        const float *pw0 = ws + block0 * ws_row, *pw1 = ws + block1 * ws_row;
-        for (int b0 = 0; b0 < blocks; b0 += kScaleGroup, ++gg) {
-          if (gg > 1 && !tc::mbar_wait(scale_empty(gg & 1), ((gg >> 1) - 1) & 1u, kWaitLimit)) {
+        const float* pw = ws + (live2 ? half * ws_row : 0);
+        for (int b0 = 0; b0 < blocks; b0 += kScaleGroup) {
+          if (use > 0 && !tc::mbar_wait(scale_empty(slot), (use - 1) & 1u, kWaitLimit)) {
             failed = true;
             break;
           }
-          float2* dst = reinterpret_cast<float2*>(base + P::kScaleOff + (gg & 1) * kScaleGroup * kScaleBlock);
-#pragma unroll 1
-          for (int q = 0; q < kScaleGroup; q += 2) {  // two blocks at a time: this warpgroup has few registers
-            float a0[2], a1[2], w0[2], w1[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int b = min(b0 + q + u, blocks - 1);
-              a0[u] = live0 ? pa0[b * as_col] : 0.f;
-              a1[u] = live1 ? pa1[b * as_col] : 0.f;
-              w0[u] = pw0[b * ws_col];
-              w1[u] = pw1[b * ws_col];
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float2* d = dst + (q + u) * 256 + i;
-              d[0] = split_scale(a0[u], w0[u]);
-              d[64] = split_scale(a1[u], w0[u]);
-              d[128] = split_scale(a0[u], w1[u]);
-              d[192] = split_scale(a1[u], w1[u]);
-            }
+          uint32_t dst = sbase + P::kScaleOff + slot * (kScaleGroup * kScaleBlock) + i * 4;
+          const int last = min(b0 + kScaleGroup, blocks);
+          for (int b = b_begin + b0; b < b_begin + last; ++b, dst += kScaleBlock) {
+            tc::cp_async4(dst, pa0 + b * as_col, live0);
+            tc::cp_async4(dst + 256, pa1 + b * as_col, live1);
+            if (i < 2) tc::cp_async4(dst + 512, pw + b * ws_col, live2);
           }
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(scale_full(gg & 1));
+          tc::cp_async_arrive(scale_full(slot));
+          if (++slot == kScaleGroups) slot = 0, ++use;
         }
       }
+      tc::cp_async_commit();
+      tc::cp_async_wait<0>();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
     const int strip = warp >> 2, quarter = warp & 3;
-    const uint32_t t0 = tmem + ((uint32_t)(quarter * 32) << 16) + strip * P::kCols;
+    const uint32_t t0 = tmem + ((uint32_t)(quarter * 32) << 16) + strip * kCols;
     uint8_t* buf4k = base + P::kStoreOff + warp * 4096;
-    const uint32_t scales = sbase + P::kScaleOff + (strip * P::kCols / kFp8Block) * 1024 + (quarter * 32 + lane) * 8;
-    uint32_t release[P::kBufs];
-#pragma unroll
-    for (int i = 0; i < P::kBufs; ++i) release[i] = tc::map_rank(acc_empty(i), 0);
+    const float* scales = reinterpret_cast<const float*>(base + P::kScaleOff);
+    const int my_row = quarter * 32 + lane, my_half = 128 + strip * kCols / kFp8Block;
+    // the issuer's acc_empty[]
+    const uint32_t release0 = tc::map_rank(acc_empty(0), kCtas == 2 ? 0 : part);
+    const uint32_t release1 = tc::map_rank(acc_empty(1), kCtas == 2 ? 0 : part);
     uint32_t g = 0, gg = 0;
-    for (int t = pair; t < tiles && !failed; t += pairs) {
+    for (int t = first; t < tiles && !failed; t += step) {
       int mt, nt;
       tile_at(t, tm, tn, mt, nt);
-      const int row0 = mt * kPairRows + rank * 128 + quarter * 32, col0 = nt * kTileN + strip * P::kCols;
-      uint64_t acc[P::kCols / 2];
+      const int row0 = (mt * kCtas + rank) * 128 + quarter * 32, col0 = nt * kTileN + strip * kCols;
+      uint64_t acc[kCols / 2];
 #pragma unroll
-      for (int j = 0; j < P::kCols / 2; ++j) acc[j] = 0;
+      for (int j = 0; j < kCols / 2; ++j) acc[j] = 0;
       for (int b0 = 0; b0 < blocks; b0 += kScaleGroup, ++gg) {
-        if (!failed && !tc::mbar_wait(scale_full(gg & 1), (gg >> 1) & 1u, kWaitLimit)) failed = true;
-        uint32_t slot = scales + (gg & 1) * kScaleGroup * kScaleBlock;
+        if (!failed && !tc::mbar_wait(scale_full(gg % kScaleGroups), (gg / kScaleGroups) & 1u, kWaitLimit)) failed = true;
+        const float* slot = scales + gg % kScaleGroups * (kScaleGroup * kScaleBlock / 4);
         const int last = min(blocks - b0, kScaleGroup);
 #pragma unroll 1
-        for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock) {
-          const uint32_t buf = g % P::kBufs;
-          if (!failed && !tc::mbar_wait(acc_full(buf), (g / P::kBufs) & 1u, kWaitLimit)) failed = true;
+        for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock / 4) {
+          const uint32_t buf = g % kAccBufs;
+          if (!failed && !tc::mbar_wait(acc_full(buf), (g / kAccBufs) & 1u, kWaitLimit)) failed = true;
           tc::fence_after_sync();
-          float pre, f;
+          float2 scale;
 #pragma unroll
-          for (int c = 0; c < P::kCols; c += 32) {
+          for (int c = 0; c < kCols; c += 32) {
             uint32_t v[32];
             tc::tmem_ld32(t0 + buf * kTileN + c, v);
-            if (c == 0) tc::ld_shared2(slot, pre, f);
+            if (c == 0) scale = split_scale(slot[my_row], slot[my_half]);
             tc::tmem_wait_ld();
-            if (c + 32 == P::kCols) {
+            if (c + 32 == kCols) {
               tc::fence_before_sync();
               __syncwarp();
-              if (lane == 0) tc::mbar_arrive_cluster(P::kBufs == 2 ? release[buf & 1] : tc::map_rank(acc_empty(buf), 0));
+              if (lane == 0) tc::mbar_arrive_cluster(buf ? release1 : release0);
             }
-            add_scaled<32>(acc + c / 2, v, pre, f);
+            add_scaled<32>(acc + c / 2, v, scale.x, scale.y);
           }
         }
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(scale_empty(gg & 1));
+        if (lane == 0) tc::mbar_arrive(scale_empty(gg % kScaleGroups));
       }
-      if (y_type == LLVQ_DT_F32)
-        store_rows<float, P::kCols>(acc, buf4k, static_cast<float*>(y), ldy, row0, col0, m_total, n_total, lane);
-      else if (y_type == LLVQ_DT_F16)
-        store_rows<__half, P::kCols>(acc, buf4k, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total, lane);
-      else
-        store_rows<__nv_bfloat16, P::kCols>(acc, buf4k, static_cast<__nv_bfloat16*>(y), ldy, row0, col0, m_total,
-                                            n_total, lane);
+      if (kCtas == 1 && splits > 1) {
+        // the last block's sums have been read by this warp, so every stage has been consumed: reuse them
+#pragma unroll
+        for (int j = 0; j < kCols / 4; ++j) {
+          float x, y_, z, w;
+          unpack2(acc[2 * j], x, y_);
+          unpack2(acc[2 * j + 1], z, w);
+          tc::st_shared4(partial_at(sbase, quarter * 32 + lane, strip * (kCols / 4) + j), x, y_, z, w);
+        }
+      } else if (y_type == LLVQ_DT_F32) {
+        store_rows<float, kCols>(acc, buf4k, static_cast<float*>(y), ldy, row0, col0, m_total, n_total, lane);
+      } else if (y_type == LLVQ_DT_F16) {
+        store_rows<__half, kCols>(acc, buf4k, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total, lane);
+      } else {
+        store_rows<__nv_bfloat16, kCols>(acc, buf4k, static_cast<__nv_bfloat16*>(y), ldy, row0, col0, m_total, n_total,
+                                         lane);
+      }
     }
   }
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
   tc::fence_before_sync();
-  tc::cluster_sync();  // no arrival or commit is under way to a CTA that has left
+  tc::cluster_sync();  // partial sums are there; no arrival or commit is under way to a CTA that has left
   tc::fence_after_sync();
-  if (warp == kAddWarps) tc::tmem_dealloc_pair(tmem, 512);
+  if (kCtas == 1 && splits > 1) {
+    if (warp < kAddWarps) {
+      int mt, nt;
+      tile_at(first, tm, tn, mt, nt);
+      const int m0 = mt * 128, n0 = nt * kTileN;
+      if (y_type == LLVQ_DT_F32)
+        store_reduced(sbase, part, splits, static_cast<float*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
+      else if (y_type == LLVQ_DT_F16)
+        store_reduced(sbase, part, splits, static_cast<__half*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
+      else
+        store_reduced(sbase, part, splits, static_cast<__nv_bfloat16*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
+    }
+    __syncwarp();
+    tc::cluster_sync();  // no CTA leaves while another still reads its sums
+  }
+  if (warp == kAddWarps + 1) tc::Ctas<kCtas>::dealloc(tmem, 512);
 }
 
 // e4m3 row-major [rows, cols] (row stride `ld` bytes), box 128 columns x
@@ -616,7 +733,7 @@ cudaError_t few_rows_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int
   const int64_t tn = (n + kTileRows - 1) / kTileRows, tm = (m + kAct - 1) / kAct;
   if (tm > 65535) return cudaErrorInvalidValue;
   // as many CTAs per tile as fit two per SM, at most a portable cluster of 8
-  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * sms / (tn * tm), 8, blocks}));
+  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * sms / (tn * tm), kMaxSplits, blocks}));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tn * splits), (unsigned)tm, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
@@ -633,34 +750,84 @@ cudaError_t few_rows_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int
                             w.scale_row, w.scale_col, m, n, y, ldy, y_type, splits, error_flag);
 }
 
-template <int kTileN>
-cudaError_t pair_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, int k, void* y, int64_t ldy,
+// Clusters of 1..kMaxSplits CTAs of Wide<1> that the current device holds at once (they have to fit its GPCs).
+cudaError_t resident_clusters(int dev, int (&held)[kMaxSplits + 1]) {
+  static std::atomic<int> cache[kMaxDevices][kMaxSplits + 1];
+  if (cache[dev][1].load(std::memory_order_acquire) == 0) {
+    for (int s = kMaxSplits; s >= 1; --s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)s, 1, 1);
+      cfg.blockDim = dim3(kWideThreads, 1, 1);
+      cfg.dynamicSmemBytes = Wide<1>::kSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)s;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, wide_kernel<1>, &cfg);
+      if (e != cudaSuccess) return e;
+      cache[dev][s].store(std::max(n, 1), std::memory_order_release);  // [1] last: the table is whole when it is set
+    }
+  }
+  for (int s = 1; s <= kMaxSplits; ++s) held[s] = cache[dev][s].load(std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+// CTAs per tile for Wide<1>: the fewest blocks in a row, over the waves of
+// clusters and the blocks of a CTA; adding the parts costs about four blocks.
+cudaError_t choose_splits(int dev, int64_t tiles, int64_t blocks, int* splits) {
+  int held[kMaxSplits + 1];
+  const cudaError_t e = resident_clusters(dev, held);
+  if (e != cudaSuccess) return e;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= kMaxSplits && s <= blocks; ++s) {
+    const int64_t waves = (tiles + held[s] - 1) / held[s], cost = waves * ((blocks + s - 1) / s + (s > 1 ? 4 : 0));
+    if (cost < best) {
+      best = cost;
+      *splits = s;
+    }
+  }
+  return cudaSuccess;
+}
+
+// Wide<1>: a tile per cluster of 1..kMaxSplits CTAs.
+template <int kCtas>
+cudaError_t wide_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, int k, void* y, int64_t ldy,
                         int y_type, int* error_flag, int sms, cudaStream_t stream) {
   static std::atomic<bool> done[kMaxDevices];
-  cudaError_t e = configure_once((const void*)pair_kernel<kTileN>, Pair<kTileN>::kSmem, done);
+  cudaError_t e = configure_once((const void*)wide_kernel<kCtas>, Wide<kCtas>::kSmem, done);
   if (e != cudaSuccess) return e;
   CUtensorMap ta, tw;
   e = encode_e4m3_map(&ta, a.q, k, m, a.ld, 128);
   if (e != cudaSuccess) return e;
-  e = encode_e4m3_map(&tw, w.q, k, n, w.ld, kTileN / 2);
+  e = encode_e4m3_map(&tw, w.q, k, n, w.ld, kTileN / kCtas);
   if (e != cudaSuccess) return e;
-  const int64_t tm = (m + (int64_t)kPairRows - 1) / kPairRows, tn = (n + (int64_t)kTileN - 1) / kTileN;
-  if (tm * tn > (1 << 30)) return cudaErrorInvalidValue;
+  const int64_t tm = (m + 128LL * kCtas - 1) / (128 * kCtas), tn = (n + (int64_t)kTileN - 1) / kTileN;
+  if (tm * tn > (1 << 27)) return cudaErrorInvalidValue;
+  int splits = 1, dev = 0;
+  if (kCtas == 1) {
+    e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    e = choose_splits(dev, tm * tn, (k + kFp8Block - 1) / kFp8Block, &splits);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tm * tn, sms / 2)), 1, 1);
-  cfg.blockDim = dim3(kPairThreads, 1, 1);
-  cfg.dynamicSmemBytes = Pair<kTileN>::kSmem;
+  cfg.gridDim = dim3((unsigned)(kCtas == 2 ? 2 * std::min<int64_t>(tm * tn, sms / 2) : tm * tn * splits), 1, 1);
+  cfg.blockDim = dim3(kWideThreads, 1, 1);
+  cfg.dynamicSmemBytes = Wide<kCtas>::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = (unsigned)(kCtas == 2 ? 2 : splits);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, pair_kernel<kTileN>, ta, tw, (k + kFp8Block - 1) / kFp8Block, a.scale, a.scale_row,
+  return cudaLaunchKernelEx(&cfg, wide_kernel<kCtas>, ta, tw, (k + kFp8Block - 1) / kFp8Block, a.scale, a.scale_row,
                             a.scale_col, w.scale, w.scale_row, w.scale_col, m, n, y, ldy, y_type, (int)tm, (int)tn,
-                            error_flag);
+                            splits, error_flag);
 }
 
 }  // namespace
@@ -675,13 +842,13 @@ cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, in
   int sms = 0;
   const cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
-#define LLVQ_FEW(N) few_rows_launch<N>(a, w, (int)m, (int)n, (int)k, y, ldy, y_type, error_flag, sms, stream)
-  if (m <= 16) return LLVQ_FEW(16);
-  if (m <= 32) return LLVQ_FEW(32);
-  if (m <= 64) return LLVQ_FEW(64);
-  if (m <= 256) return LLVQ_FEW(128);
-  return pair_launch<256>(a, w, (int)m, (int)n, (int)k, y, ldy, y_type, error_flag, sms, stream);
-#undef LLVQ_FEW
+#define LLVQ_CALL a, w, (int)m, (int)n, (int)k, y, ldy, y_type, error_flag, sms
+  if (m <= 16) return few_rows_launch<16>(LLVQ_CALL, stream);
+  if (m <= 32) return few_rows_launch<32>(LLVQ_CALL, stream);
+  if (m <= 64) return few_rows_launch<64>(LLVQ_CALL, stream);
+  const int64_t tiles = (m + 127) / 128 * ((n + kTileN - 1) / kTileN);
+  return tiles > sms ? wide_launch<2>(LLVQ_CALL, stream) : wide_launch<1>(LLVQ_CALL, stream);
+#undef LLVQ_CALL
 }
 
 }  // namespace llvq

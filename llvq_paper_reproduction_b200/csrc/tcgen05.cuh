@@ -176,8 +176,9 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 __device__ __forceinline__ void cp_async4(uint32_t saddr, const void* p, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(saddr), "l"(p), "r"(live ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void ld_shared2(uint32_t saddr, float& a, float& b) {
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(saddr) : "memory");
+// Arrive on the mbarrier once this thread's copies so far are there (one of the arrivals it counts).
+__device__ __forceinline__ void cp_async_arrive(uint32_t mbar_saddr) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(mbar_saddr) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -241,6 +242,49 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_saddr, const void*
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mbar_cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mbar_cluster_addr) : "memory");
 }
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared4(uint32_t saddr, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(saddr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+
+// The same calls for a CTA alone (1) and for a pair (2).
+template <int kCtas>
+struct Ctas;
+
+template <>
+struct Ctas<1> {
+  static __device__ __forceinline__ void alloc(uint32_t holder, uint32_t n) { tmem_alloc(holder, n); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tmem_dealloc(t, n); }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    mma_f8(d, a, b, idesc, acc);
+  }
+  static __device__ __forceinline__ void commit(uint32_t bar) { tc::commit(bar); }
+  static __device__ __forceinline__ void tma_load(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    tma_load_2d(dst, map, x, y, bar);
+  }
+};
+
+template <>
+struct Ctas<2> {
+  static __device__ __forceinline__ void alloc(uint32_t holder, uint32_t n) { tmem_alloc_pair(holder, n); }
+  static __device__ __forceinline__ void dealloc(uint32_t t, uint32_t n) { tmem_dealloc_pair(t, n); }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    mma_f8_pair(d, a, b, idesc, acc);
+  }
+  static __device__ __forceinline__ void commit(uint32_t bar) { commit_pair(bar); }
+  static __device__ __forceinline__ void tma_load(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    tma_load_2d_pair(dst, map, x, y, bar);
+  }
+};
 
 }  // namespace tc
 }  // namespace llvq
