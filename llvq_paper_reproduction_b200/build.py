@@ -23,6 +23,9 @@ CSRC = PKG / "csrc"
 GEN = CSRC / "_gen" / "search_gen.cuh"
 BUILD = PKG / "_build"
 LIB = PKG / "_lib" / "libllvq_b200.so"
+# Tensor front end of the 8-bit operators: a CPython module against the installed torch.
+TORCH_SRC = CSRC / "fp8_torch.cpp"
+TORCH_EXT = PKG / "_lib" / "_fp8_torch.so"
 INCLUDE = PKG.parent / "include"
 
 # Codebooks with generated search code: name, min shell, max shell.
@@ -67,6 +70,32 @@ def _compile(src: Path, obj: Path, verbose: bool) -> str:
     return res.stderr
 
 
+def build_torch_extension(force: bool = False) -> Path:
+    """Compile fp8_torch.cpp with the host compiler against the torch that is
+    installed; again when it, the public header or torch itself is newer."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    newest = max(p.stat().st_mtime for p in (TORCH_SRC, INCLUDE / "llvq_b200.h", root / "version.py"))
+    if force or not TORCH_EXT.exists() or TORCH_EXT.stat().st_mtime < newest:
+        cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+        cuda = Path(nvcc()).resolve().parent.parent / "include"
+        tmp = TORCH_EXT.with_name(TORCH_EXT.name + ".tmp")
+        abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+               "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+               "-I", sysconfig.get_paths()["include"], "-I", str(cuda), "-I", str(INCLUDE), str(TORCH_SRC), "-o",
+               str(tmp), "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+               "-ltorch_python"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode:
+            raise RuntimeError(f"{cxx} failed for {TORCH_SRC.name}:\n{res.stderr}")
+        tmp.replace(TORCH_EXT)
+    return TORCH_EXT
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
     generate()
     BUILD.mkdir(exist_ok=True)
@@ -89,6 +118,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         tmp = LIB.with_name(LIB.name + ".tmp")
         subprocess.run([nvcc(), *ARCH, "-shared", "-o", str(tmp), *map(str, objs)], check=True)
         tmp.replace(LIB)
+    build_torch_extension(force)
     if verbose:
         for name, log in sorted(logs.items()):
             print(f"== {name}\n{log}")
