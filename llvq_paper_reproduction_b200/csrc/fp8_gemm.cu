@@ -40,10 +40,78 @@ __device__ __forceinline__ T to_out(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ void store_out(void* y, int64_t i, float v, int type) {
-  if (type == LLVQ_DT_F32) static_cast<float*>(y)[i] = v;
-  else if (type == LLVQ_DT_F16) static_cast<__half*>(y)[i] = to_out<__half>(v);
-  else static_cast<__nv_bfloat16*>(y)[i] = to_out<__nv_bfloat16>(v);
+// Four neighbouring outputs, `count` of them in the matrix; whole: 16-byte stores are possible.
+__device__ __forceinline__ void store4(void* y, int64_t i, float4 v, int type, bool whole, int count) {
+  if (type == LLVQ_DT_F32) {
+    float* p = static_cast<float*>(y) + i;
+    if (whole && count >= 4) {
+      *reinterpret_cast<float4*>(p) = v;
+    } else {
+      p[0] = v.x;
+      if (count > 1) p[1] = v.y;
+      if (count > 2) p[2] = v.z;
+      if (count > 3) p[3] = v.w;
+    }
+    return;
+  }
+  uint2 w;
+  if (type == LLVQ_DT_F16) {
+    const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
+  uint16_t* p = static_cast<uint16_t*>(y) + i;
+  if (whole && count >= 4) {
+    *reinterpret_cast<uint2*>(p) = w;
+  } else {
+    p[0] = (uint16_t)w.x;
+    if (count > 1) p[1] = (uint16_t)(w.x >> 16);
+    if (count > 2) p[2] = (uint16_t)w.y;
+    if (count > 3) p[3] = (uint16_t)(w.y >> 16);
+  }
+}
+
+// Whether rows of y can be stored in 16-byte chunks.
+__device__ __forceinline__ bool whole_chunks(const void* y, int64_t ldy, int type) {
+  const int64_t size = type == LLVQ_DT_F32 ? 4 : 2;
+  return ldy * size % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+}
+
+// Partial sums of a tile in shared memory: rows of kWidth fp32 in 16-byte chunks, kSwizzle: exchanged by the row.
+template <int kWidth, bool kSwizzle>
+__device__ __forceinline__ uint32_t partial_at(uint32_t base, int row, int chunk) {
+  return base + (uint32_t)row * (kWidth * 4) + (uint32_t)((kSwizzle ? chunk ^ (row & 7) : chunk) * 16);
+}
+
+// Adds the tile's parts over the cluster in rank order and stores them; this
+// CTA takes a 1 / splits share.  Rolled loops: this runs once, and straight
+// code costs more to fetch (about two cycles a byte: an unrolled form took 9300
+// cycles of a 20,000-cycle kernel) than its loads take one after the other.
+template <int kWidth, bool kSwizzle>
+__device__ __forceinline__ void store_reduced(uint32_t partial, int rank, int splits, void* y, int64_t ldy, int y_type,
+                                              int m0, int n0, int rows, int n_total, int t, int threads) {
+  constexpr int kChunks = kWidth / 4;
+  const bool whole = whole_chunks(y, ldy, y_type);
+  const int all = rows * kChunks, end = all * (rank + 1) / splits;
+#pragma unroll 1
+  for (int e = all * rank / splits + t; e < end; e += threads) {
+    const int r = e / kChunks, chunk = e % kChunks, col = n0 + chunk * 4;
+    if (col >= n_total) continue;
+    const uint32_t at = partial_at<kWidth, kSwizzle>(partial, r, chunk);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int s = 0; s < splits; s += 4) {
+      float4 p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[i] = s + i < splits ? tc::ld_cluster4(tc::map_rank(at, s + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum.x += p[i].x, sum.y += p[i].y, sum.z += p[i].z, sum.w += p[i].w;
+    }
+    store4(y, (int64_t)(m0 + r) * ldy + col, sum, y_type, whole, n_total - col);
+  }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -229,37 +297,19 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         }
       }
     }
-    const int n = n0 + (warp & 3) * 32 + lane;
-    if (splits == 1) {
+    // the last block's sums have been read, so every stage has been consumed: reuse them
+    float* part = reinterpret_cast<float*>(base) + (warp & 3) * 32 + lane;
 #pragma unroll
-      for (int j = 0; j < kAct; ++j)
-        if (n < n_total && m0 + j < m_total) store_out(y, (int64_t)(m0 + j) * ldy + n, acc[j], y_type);
-    } else {
-      // the last block's sums have been read, so every stage has been consumed: reuse them
-      float* red = reinterpret_cast<float*>(base);
-#pragma unroll
-      for (int j = 0; j < kAct; ++j) red[j * kTileRows + (warp & 3) * 32 + lane] = acc[j];
-    }
+    for (int j = 0; j < kAct; ++j) part[j * kTileRows] = acc[j];
   }
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
-  if (splits > 1) {
-    tc::cluster_sync();
-    if (warp >= 2) {  // CTA `rank` adds activation rows rank, rank + splits, ...
-      const int t = tid - 64, n = n0 + t;
-      for (int j = rank; j < kAct && m0 + j < m_total; j += splits) {
-        const uint32_t at = sbase + (uint32_t)(j * kTileRows + t) * 4;
-        float part[kMaxSplits], sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < kMaxSplits; ++r) part[r] = r < splits ? tc::ld_cluster(tc::map_rank(at, r)) : 0.f;
-#pragma unroll
-        for (int r = 0; r < kMaxSplits; ++r) sum += part[r];  // the zeros past splits change nothing
-        if (n < n_total) store_out(y, (int64_t)(m0 + j) * ldy + n, sum, y_type);
-      }
-    }
-    __syncwarp();
-    tc::cluster_sync();  // no CTA leaves while another still reads its sums
-  }
+  tc::cluster_sync();
+  if (warp >= 2)
+    store_reduced<kTileRows, false>(sbase, rank, splits, y, ldy, y_type, m0, n0, min(kAct, m_total - m0), n_total,
+                                    tid - 64, 128);
+  __syncwarp();
+  tc::cluster_sync();  // no CTA leaves while another still reads its sums
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -351,12 +401,6 @@ __device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, float pre
   for (int j = 0; j < kCount / 2; ++j) acc[j] = fma2(pack2(v[2 * j], v[2 * j + 1]), ff, acc[j]);
 }
 
-// y as rows of 16-byte chunks where its base and stride allow.
-template <typename T>
-__device__ __forceinline__ bool whole_chunks(const T* y, int64_t ldy) {
-  return ldy * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-}
-
 // A warp's 32 rows x kWidth columns to y, through its 4 KB of shared memory (32
 // rows of 128 bytes, 16-byte chunks swizzled by the row) so that the global
 // stores are whole 128-byte lines.
@@ -364,7 +408,7 @@ template <typename T, int kWidth>
 __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0,
                                            int col0, int m_total, int n_total, int lane) {
   constexpr int kPerLine = 128 / (int)sizeof(T), kPerChunk = 16 / (int)sizeof(T);
-  const bool whole = whole_chunks(y, ldy);
+  const bool whole = ldy * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
 #pragma unroll
   for (int c0 = 0; c0 < kWidth; c0 += kPerLine) {
 #pragma unroll
@@ -380,20 +424,39 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T*
       *reinterpret_cast<uint4*>(buf + lane * 128 + ((ch ^ (lane & 7)) * 16)) = *reinterpret_cast<const uint4*>(e);
     }
     __syncwarp();
+    if (whole) {
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int r = it * 4 + (lane >> 3), ch = lane & 7;
-      const int row = row0 + r, col = col0 + c0 + ch * kPerChunk;
-      const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 128 + ((ch ^ (r & 7)) * 16));
-      if (row < m_total && col < n_total) {
-        T* dst = y + (int64_t)row * ldy + col;
-        if (whole && col + kPerChunk <= n_total) {
-          *reinterpret_cast<uint4*>(dst) = v;
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 4 + (lane >> 3), ch = lane & 7;
+        const int row = row0 + r, col = col0 + c0 + ch * kPerChunk;
+        const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 128 + ((ch ^ (r & 7)) * 16));
+        if (row < m_total && col < n_total) {  // 
+          T* dst = y + (int64_t)row * ldy + col;
+          if (col + kPerChunk <= n_total) {
+            *reinterpret_cast<uint4*>(dst) = v;
+          } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int j = 0; j < kPerChunk; ++j)
+              if (col + j < n_total) dst[j] = e[j];
+          }
+        }
+      }
+    } else {  // rows off 16-byte boundaries: a row of the buffer at a time, four bytes a lane
+      constexpr int kPerWord = 4 / (int)sizeof(T);
+      const int col = col0 + c0 + lane * kPerWord;
+      const bool words = ldy * (int64_t)sizeof(T) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0;
+#pragma unroll 4
+      for (int r = 0; r < 32; ++r) {
+        if (row0 + r >= m_total || col >= n_total) break;
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+        T* dst = y + (int64_t)(row0 + r) * ldy + col;
+        if (words && col + kPerWord <= n_total) {
+          *reinterpret_cast<uint32_t*>(dst) = v;
         } else {
           const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-          for (int j = 0; j < kPerChunk; ++j)
-            if (col + j < n_total) dst[j] = e[j];
+          dst[0] = e[0];
+          if (kPerWord > 1 && col + 1 < n_total) dst[kPerWord - 1] = e[kPerWord - 1];
         }
       }
     }
@@ -408,49 +471,6 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& mt, int& nt)
   const int height = min(16, tm - group * 16);
   mt = group * 16 + in % height;
   nt = in / height;
-}
-
-// Partial sums of a tile in shared memory: rows of 256 fp32, 16-byte chunks swizzled by the row.
-__device__ __forceinline__ uint32_t partial_at(uint32_t base, int row, int chunk) {
-  return base + (uint32_t)row * (kTileN * 4) + (uint32_t)((chunk ^ (row & 7)) * 16);
-}
-
-// This CTA's rows (a 1 / splits share) of the tile, added over the cluster in rank order.
-template <typename T>
-__device__ __forceinline__ void store_reduced(uint32_t partial, int rank, int splits, T* __restrict__ y, int64_t ldy,
-                                              int m0, int n0, int m_total, int n_total, int warp, int lane) {
-  const bool whole = whole_chunks(y, ldy);
-  const int end = min((rank + 1) * 128 / splits, m_total - m0);
-  for (int r = rank * 128 / splits + warp; r < end; r += kAddWarps) {
-#pragma unroll
-    for (int c = 0; c < kTileN / 128; ++c) {
-      const int chunk = c * 32 + lane, col = n0 + chunk * 4;
-      if (col >= n_total) continue;
-      float4 part[kMaxSplits], sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s)  // all the reads under way before the first sum
-        part[s] = s < splits ? tc::ld_cluster4(tc::map_rank(partial_at(partial, r, chunk), s))
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s)
-        sum.x += part[s].x, sum.y += part[s].y, sum.z += part[s].z, sum.w += part[s].w;
-      T e[4] = {to_out<T>(sum.x), to_out<T>(sum.y), to_out<T>(sum.z), to_out<T>(sum.w)};
-      T* dst = y + (int64_t)(m0 + r) * ldy + col;
-      if (whole && col + 4 <= n_total) {
-        if constexpr (sizeof(T) == 4) {
-          *reinterpret_cast<float4*>(dst) = make_float4(e[0], e[1], e[2], e[3]);
-        } else {
-          uint2 w;
-          memcpy(&w, e, 8);
-          *reinterpret_cast<uint2*>(dst) = w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < n_total) dst[j] = e[j];
-      }
-    }
-  }
 }
 
 // Wide<2>: `split` is 1 and a pair takes tiles pair, + pairs, ...  Wide<1>: one
@@ -656,7 +676,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           float x, y_, z, w;
           unpack2(acc[2 * j], x, y_);
           unpack2(acc[2 * j + 1], z, w);
-          tc::st_shared4(partial_at(sbase, quarter * 32 + lane, strip * (kCols / 4) + j), x, y_, z, w);
+          tc::st_shared4(partial_at<kTileN, true>(sbase, my_row, strip * (kCols / 4) + j), x, y_, z, w);
         }
       } else if (y_type == LLVQ_DT_F32) {
         store_rows<float, kCols>(acc, buf4k, static_cast<float*>(y), ldy, row0, col0, m_total, n_total, lane);
@@ -677,13 +697,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if (warp < kAddWarps) {
       int mt, nt;
       tile_at(first, tm, tn, mt, nt);
-      const int m0 = mt * 128, n0 = nt * kTileN;
-      if (y_type == LLVQ_DT_F32)
-        store_reduced(sbase, part, splits, static_cast<float*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
-      else if (y_type == LLVQ_DT_F16)
-        store_reduced(sbase, part, splits, static_cast<__half*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
-      else
-        store_reduced(sbase, part, splits, static_cast<__nv_bfloat16*>(y), ldy, m0, n0, m_total, n_total, warp, lane);
+      store_reduced<kTileN, true>(sbase, part, splits, y, ldy, y_type, mt * 128, nt * kTileN,
+                                  min(128, m_total - mt * 128), n_total, tid, kAddWarps * 32);
     }
     __syncwarp();
     tc::cluster_sync();  // no CTA leaves while another still reads its sums
@@ -775,15 +790,17 @@ cudaError_t resident_clusters(int dev, int (&held)[kMaxSplits + 1]) {
   return cudaSuccess;
 }
 
-// CTAs per tile for Wide<1>: the fewest blocks in a row, over the waves of
-// clusters and the blocks of a CTA; adding the parts costs about four blocks.
+// CTAs per tile for Wide<1>: the shortest time over the waves of clusters, in
+// blocks (850 cycles each): a wave starts and stores in about 9, and adding the
+// parts takes 10 more (11,500 cycles for 128 rows, most of them the reads of
+// distributed shared memory).
 cudaError_t choose_splits(int dev, int64_t tiles, int64_t blocks, int* splits) {
   int held[kMaxSplits + 1];
   const cudaError_t e = resident_clusters(dev, held);
   if (e != cudaSuccess) return e;
   int64_t best = INT64_MAX;
   for (int s = 1; s <= kMaxSplits && s <= blocks; ++s) {
-    const int64_t waves = (tiles + held[s] - 1) / held[s], cost = waves * ((blocks + s - 1) / s + (s > 1 ? 4 : 0));
+    const int64_t waves = (tiles + held[s] - 1) / held[s], cost = waves * ((blocks + s - 1) / s + (s > 1 ? 19 : 9));
     if (cost < best) {
       best = cost;
       *splits = s;
