@@ -21,6 +21,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "fp8_launch.cuh"
 #include "llvq_b200.h"
 #include "llvq_internal.h"
 
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* __restrict__
                                                            const T* __restrict__ up, int64_t ldu, uint32_t rows,
                                                            uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
                                                            int64_t cols, Fp8Out out) {
+  dependents_may_start();
   constexpr int kUnits = kRowUnits<T, kGated>;
   constexpr int kTeams = kRowThreads / kGroup;
   const uint32_t first = blockIdx.x * (kTeams * kUnits) + threadIdx.x / kGroup;
@@ -309,6 +311,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* __restrict__
   uint32_t row[kUnits], b[kUnits];
   int valid[kUnits];
   Raw<T> rx[kUnits], ru[kUnits];
+  wait_for_inputs();
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
     if (j == 0) {
@@ -354,12 +357,14 @@ constexpr int kBlockPasses = kFp8Block / kBlockRowsPass;     // 4
 template <typename T, int kStep>
 __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                                int64_t cols, uint32_t col_blocks, Fp8Out out) {
+  dependents_may_start();
   __shared__ float red[kBlockThreads / 32];
   const uint32_t rb = blockIdx.x / col_blocks, cb = blockIdx.x % col_blocks;
   const int64_t c = (int64_t)cb * kFp8Block + (threadIdx.x % kGroup) * kVec;
   const int64_t r0 = (int64_t)rb * kFp8Block + threadIdx.x / kGroup;
   const int valid = valid_of(cols, c);
   Raw<T> raw[kBlockPasses];
+  wait_for_inputs();
 #pragma unroll
   for (int p = 0; p < kBlockPasses; ++p) {
     const int64_t r = r0 + p * kBlockRowsPass;
@@ -405,6 +410,7 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 80 : 64)
                     const W* __restrict__ weight, float eps, float inv_cols, int64_t rows, int64_t cols,
                     T* __restrict__ hidden, int64_t ldh, Fp8Out out) {
   constexpr bool kAhead = kThreads == 512 && sizeof(T) == 2;  // fp32 rows would spill
+  dependents_may_start();
   __shared__ float red[2][32];
   Raw<T> rx[kChunks], rr[kChunks];
   auto load = [&](int64_t row) {
@@ -416,6 +422,7 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 80 : 64)
       if constexpr (kResidual) rr[j] = load_vec<T, kStep>(residual + (valid ? row * ldr + c : 0), valid);
     }
   };
+  wait_for_inputs();
   if constexpr (kAhead) load(blockIdx.x);
   int side = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, side ^= 1) {
@@ -483,10 +490,10 @@ cudaError_t rows_step(Fp8In x, Fp8In up, int64_t rows, int64_t cols, Fp8Out out,
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block, units = rows * blocks;
   constexpr int kTeams = kRowThreads / kGroup, kCta = kTeams * kRowUnits<T, kGated>;
   if (units > 0xFFFFFFFFLL - kCta) return cudaErrorInvalidValue;
-  rows_kernel<T, kGated, kStep><<<(unsigned)((units + kCta - 1) / kCta), kRowThreads, 0, stream>>>(
-      static_cast<const T*>(x.ptr), x.ld, static_cast<const T*>(up.ptr), up.ld, (uint32_t)rows, (uint32_t)blocks,
-      (uint32_t)(kTeams / blocks), (uint32_t)(kTeams % blocks), cols, out);
-  return cudaGetLastError();
+  return launch_overlapped(rows_kernel<T, kGated, kStep>, dim3((unsigned)((units + kCta - 1) / kCta)), kRowThreads, 0, 0,
+                           stream, static_cast<const T*>(x.ptr), x.ld, static_cast<const T*>(up.ptr), up.ld,
+                           (uint32_t)rows, (uint32_t)blocks, (uint32_t)(kTeams / blocks), (uint32_t)(kTeams % blocks),
+                           cols, out);
 }
 
 template <typename T, bool kGated>
@@ -503,14 +510,12 @@ cudaError_t blocks_typed(Fp8In x, int64_t rows, int64_t cols, Fp8Out out, cudaSt
   const int64_t rb = (rows + kFp8Block - 1) / kFp8Block, cb = (cols + kFp8Block - 1) / kFp8Block;
   if (rb * cb > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
   const T* px = static_cast<const T*>(x.ptr);
-#define LLVQ_BLOCKS(S) \
-  blocks_kernel<T, S><<<(unsigned)(rb * cb), kBlockThreads, 0, stream>>>(px, x.ld, rows, cols, (uint32_t)cb, out)
+#define LLVQ_BLOCKS(S)                                                                                         \
+  launch_overlapped(blocks_kernel<T, S>, dim3((unsigned)(rb * cb)), kBlockThreads, 0, 0, stream, px, x.ld, rows, cols, \
+                    (uint32_t)cb, out)
   const int step = step_of<T>(px, x.ld, cols);
-  if (step == 8) LLVQ_BLOCKS(8);
-  else if (step == 4) LLVQ_BLOCKS(4);
-  else LLVQ_BLOCKS(1);
+  return step == 8 ? LLVQ_BLOCKS(8) : step == 4 ? LLVQ_BLOCKS(4) : LLVQ_BLOCKS(1);
 #undef LLVQ_BLOCKS
-  return cudaGetLastError();
 }
 
 struct NormCall {
@@ -533,11 +538,10 @@ cudaError_t norm_step(const NormCall& n) {
   const cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
   const int64_t resident = (int64_t)sms * std::max(1, (kChunks == 1 ? 1024 : 704) / threads);  // one wave
-  kernel<<<(unsigned)std::min(n.rows, resident), threads, 0, n.stream>>>(
-      static_cast<const T*>(n.x.ptr), n.x.ld, static_cast<const T*>(n.residual.ptr), n.residual.ld,
-      static_cast<const W*>(n.weight), n.eps, 1.f / (float)n.cols, n.rows, n.cols,
-      static_cast<T*>(n.hidden), n.ldh, n.out);
-  return cudaGetLastError();
+  return launch_overlapped(kernel, dim3((unsigned)std::min(n.rows, resident)), threads, 0, 0, n.stream,
+                           static_cast<const T*>(n.x.ptr), n.x.ld, static_cast<const T*>(n.residual.ptr), n.residual.ld,
+                           static_cast<const W*>(n.weight), n.eps, 1.f / (float)n.cols, n.rows, n.cols,
+                           static_cast<T*>(n.hidden), n.ldh, n.out);
 }
 
 template <typename T, typename W, int kChunks, int kThreads>
