@@ -190,7 +190,9 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     tc::mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::fence_proxy_async();
-    // the first loads are under way while the CTA sets up
+    // the first loads are under way while the CTA sets up, the weights' on their way to L2 even before the
+    // kernel ahead of this one has ended
+    for (int i = 0; i < F::kStages && i < count; ++i) tc::tma_prefetch_2d(&tw, (b_begin + i) * kFp8Block, n0);
     wait_for_inputs();
     for (int i = 0; i < F::kStages && i < count; ++i) load_stage(i);
   }
@@ -744,6 +746,15 @@ cudaError_t configure_once(const void* kernel, size_t smem, std::atomic<bool>* d
   return e;
 }
 
+// CTAs per tile: one CTA per SM where a number of them comes near that (32
+// tiles: 4; 16: 8), else as many as fit two per SM (86 tiles: 3).  4096 x 4096 at
+// m = 1: 4 CTAs a tile 6.8 us, 8 7.4; 11008 x 4096: 3 CTAs 11.4, 1 12.8.
+int few_splits(int64_t tiles, int64_t blocks, int sms) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({2 * sms / tiles, kMaxSplits, blocks}));
+  const int64_t one_each = std::min(sms / tiles, most);
+  return (int)(one_each > 0 && one_each * tiles * 20 >= 17 * sms ? one_each : most);
+}
+
 template <int kAct>
 cudaError_t few_rows_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, int k, void* y, int64_t ldy,
                             int y_type, int* error_flag, int sms, cudaStream_t stream) {
@@ -758,15 +769,16 @@ cudaError_t few_rows_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int
   const int blocks = (k + kFp8Block - 1) / kFp8Block;
   const int64_t tn = (n + kTileRows - 1) / kTileRows, tm = (m + kAct - 1) / kAct;
   if (tm > 65535) return cudaErrorInvalidValue;
-  // CTAs per tile: about one CTA per SM where a number of them comes near that (32 tiles: 4; 16: 8), else as
-  // many as fit two per SM (86 tiles: 3).  4096 x 4096 at m = 1: 4 CTAs a tile 6.8 us, 8 7.4; 11008 x 4096: 3
-  // CTAs 11.4, 1 12.8.
-  const int64_t tiles = tn * tm, most = std::max<int64_t>(1, std::min<int64_t>({2 * sms / tiles, kMaxSplits, blocks}));
-  const int64_t one_each = std::min(sms / tiles, most);
-  const int splits = (int)(one_each > 0 && one_each * tiles * 20 >= 17 * sms ? one_each : most);
+  const int splits = few_splits(tn * tm, blocks, sms);
   return launch_overlapped(few_rows_kernel<kAct>, dim3((unsigned)(tn * splits), (unsigned)tm), kFewThreads,
                            Few<kAct>::kSmem, splits, stream, tw, ta, blocks, a.scale, a.scale_row, a.scale_col,
                            w.scale, w.scale_row, w.scale_col, m, n, y, ldy, y_type, splits, error_flag);
+}
+
+template <int kCtas>
+cudaError_t configure_wide() {
+  static std::atomic<bool> done[kMaxDevices];
+  return configure_once((const void*)wide_kernel<kCtas>, Wide<kCtas>::kSmem, done);
 }
 
 // Clusters of 1..kMaxSplits CTAs of Wide<1> that the current device holds at once (they have to fit its GPCs).
@@ -795,30 +807,35 @@ cudaError_t resident_clusters(int dev, int (&held)[kMaxSplits + 1]) {
 }
 
 // CTAs per tile for Wide<1>: the shortest time over the waves of clusters, in
-// blocks (850 cycles each): a wave starts and stores in about 9, and adding the
-// parts takes 10 more (11,500 cycles for 128 rows, most of them the reads of
-// distributed shared memory).
-cudaError_t choose_splits(int dev, int64_t tiles, int64_t blocks, int* splits) {
-  int held[kMaxSplits + 1];
-  const cudaError_t e = resident_clusters(dev, held);
+// cycles as measured: 850 a block, a wave starts and stores in about 9 blocks'
+// time, and adding the parts takes 10 more (11,500 cycles for 128 rows, most of
+// them the reads of distributed shared memory).
+cudaError_t choose_splits(int64_t tiles, int64_t blocks, int* splits, int64_t* cycles) {
+  int dev = 0, held[kMaxSplits + 1];
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  int64_t best = INT64_MAX;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  e = configure_wide<1>();
+  if (e != cudaSuccess) return e;
+  e = resident_clusters(dev, held);
+  if (e != cudaSuccess) return e;
+  *cycles = INT64_MAX;
   for (int s = 1; s <= kMaxSplits && s <= blocks; ++s) {
-    const int64_t waves = (tiles + held[s] - 1) / held[s], cost = waves * ((blocks + s - 1) / s + (s > 1 ? 19 : 9));
-    if (cost < best) {
-      best = cost;
+    const int64_t waves = (tiles + held[s] - 1) / held[s];
+    const int64_t cost = 850 * waves * ((blocks + s - 1) / s + (s > 1 ? 19 : 9));
+    if (cost < *cycles) {
+      *cycles = cost;
       *splits = s;
     }
   }
   return cudaSuccess;
 }
 
-// Wide<1>: a tile per cluster of 1..kMaxSplits CTAs.
+// splits: CTAs per tile (Wide<1>).
 template <int kCtas>
 cudaError_t wide_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, int k, void* y, int64_t ldy,
-                        int y_type, int* error_flag, int sms, cudaStream_t stream) {
-  static std::atomic<bool> done[kMaxDevices];
-  cudaError_t e = configure_once((const void*)wide_kernel<kCtas>, Wide<kCtas>::kSmem, done);
+                        int y_type, int* error_flag, int sms, int splits, cudaStream_t stream) {
+  cudaError_t e = configure_wide<kCtas>();
   if (e != cudaSuccess) return e;
   CUtensorMap ta, tw;
   e = encode_e4m3_map(&ta, a.q, k, m, a.ld, 128);
@@ -827,13 +844,6 @@ cudaError_t wide_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, 
   if (e != cudaSuccess) return e;
   const int64_t tm = (m + 128LL * kCtas - 1) / (128 * kCtas), tn = (n + (int64_t)kTileN - 1) / kTileN;
   if (tm * tn > (1 << 27)) return cudaErrorInvalidValue;
-  int splits = 1, dev = 0;
-  if (kCtas == 1) {
-    e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    e = choose_splits(dev, tm * tn, (k + kFp8Block - 1) / kFp8Block, &splits);
-    if (e != cudaSuccess) return e;
-  }
   const int64_t grid = kCtas == 2 ? 2 * std::min<int64_t>(tm * tn, sms / 2) : tm * tn * splits;
   return launch_overlapped(wide_kernel<kCtas>, dim3((unsigned)grid), kWideThreads, Wide<kCtas>::kSmem,
                            kCtas == 2 ? 2 : splits, stream, ta, tw, (k + kFp8Block - 1) / kFp8Block, a.scale,
@@ -851,14 +861,28 @@ cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, in
     return cudaMemset2DAsync(y, (size_t)ldy * size, 0, (size_t)n * size, (size_t)m, stream);
   }
   int sms = 0;
-  const cudaError_t e = device_sms(&sms);
+  cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
 #define LLVQ_CALL a, w, (int)m, (int)n, (int)k, y, ldy, y_type, error_flag, sms
   if (m <= 16) return few_rows_launch<16>(LLVQ_CALL, stream);
   if (m <= 32) return few_rows_launch<32>(LLVQ_CALL, stream);
   if (m <= 64) return few_rows_launch<64>(LLVQ_CALL, stream);
-  const int64_t tiles = (m + 127) / 128 * ((n + kTileN - 1) / kTileN);
-  return tiles > sms ? wide_launch<2>(LLVQ_CALL, stream) : wide_launch<1>(LLVQ_CALL, stream);
+  const int64_t blocks = (k + kFp8Block - 1) / kFp8Block, tiles = (m + 127) / 128 * ((n + kTileN - 1) / kTileN);
+  if (tiles > sms) return wide_launch<2>(LLVQ_CALL, 1, stream);
+  int splits = 1;
+  int64_t cycles = 0;
+  e = choose_splits(tiles, blocks, &splits, &cycles);
+  if (e != cudaSuccess) return e;
+  // Tiles of 64 activation rows take 7500 cycles and 800 a block while the SMs
+  // hold one CTA each: shorter where the wide tiles would be few and their parts
+  // many.  128 x 4096 x 4096: 11.6 us against 14.1; 128 x 4096 x 14336: 26.8
+  // against 21.1; 512 x 1024 x 4096: 11.4 against 13.4.
+  const int64_t few = (m + 63) / 64 * ((n + kTileRows - 1) / kTileRows);
+  if (2 * few <= sms) {
+    const int s = few_splits(few, blocks, sms);
+    if (7500 + 800 * ((blocks + s - 1) / s) < cycles) return few_rows_launch<64>(LLVQ_CALL, stream);
+  }
+  return wide_launch<1>(LLVQ_CALL, splits, stream);
 #undef LLVQ_CALL
 }
 

@@ -84,6 +84,13 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_saddr, const void* tmap
       : "memory");
 }
 
+// Bring a tile into L2 (a hint: L2 is coherent, so what is written there later is what a load reads).
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(tmap)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
 // Wait for phase `parity` of an mbarrier, giving up after `limit` polls.
 // Returns false on timeout.
 __device__ __forceinline__ bool mbar_wait(uint32_t mbar_saddr, uint32_t parity, uint32_t limit) {
