@@ -31,7 +31,6 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // gemm.cu
 
 namespace {
 
-constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr int kMaxSplits = 8;  // CTAs that share a tile's K blocks: a portable cluster
 
 template <typename T>
@@ -209,7 +208,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (lane == 0) {  // TMA producer
       int i = F::kStages;
       for (; i < count; ++i) {
-        if (!tc::mbar_wait(empty(i % F::kStages), (i / F::kStages - 1) & 1, kWaitLimit)) {
+        if (!tc::mbar_wait_asleep(empty(i % F::kStages), (i / F::kStages - 1) & 1)) {
           failed = true;
           break;
         }
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       // no copy may still be in flight when the block exits: wait for the last use of every stage
       i = min(i, count);
       for (int u = i > F::kStages ? i - F::kStages : 0; u < i; ++u)
-        tc::mbar_wait(full(u % F::kStages), (u / F::kStages) & 1, kWaitLimit);
+        tc::mbar_wait_asleep(full(u % F::kStages), (u / F::kStages) & 1);
     }
   } else if (warp == 1) {  // MMA issuer: the warp waits, one thread issues
     constexpr uint32_t idesc = tc::idesc_e4m3_f32(kTileRows, kAct);
@@ -227,8 +226,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     uint32_t st = 0, st_use = 0;
     for (int i = 0; i < count; ++i) {
       const uint32_t in_group = i % F::kGroup, buf = i / F::kGroup % F::kBufs, use = i / F::kGroup / F::kBufs;
-      if ((in_group == 0 && use > 0 && !tc::mbar_wait(acc_empty(buf), (use - 1) & 1u, kWaitLimit)) ||
-          !tc::mbar_wait(full(st), st_use & 1u, kWaitLimit)) {
+      if ((in_group == 0 && use > 0 && !tc::mbar_wait_asleep(acc_empty(buf), (use - 1) & 1u)) ||
+          !tc::mbar_wait_asleep(full(st), st_use & 1u)) {
         failed = true;
         break;
       }
@@ -247,7 +246,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // every MMA issued has finished before TMEM is freed
     if (issuer) tc::commit(drain);
     __syncwarp();
-    tc::mbar_wait(drain, 0, kWaitLimit);
+    tc::mbar_wait_asleep(drain, 0);
   } else {  // warps 2..5 read TMEM lane quarters 2, 3, 0, 1
     const int t = tid - 64;
     const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -276,7 +275,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         if (i0 + F::kChunk < count) fetch(i0 / F::kChunk + 1);
       }
       const int buf = i0 / F::kGroup % F::kBufs;
-      if (!failed && !tc::mbar_wait(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1, kWaitLimit)) failed = true;
+      if (!failed && !tc::mbar_wait_asleep(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1)) failed = true;
       tc::fence_after_sync();
       const float* slot = scales + (i0 / F::kChunk & 1) * F::kScaleFloats + i0 % F::kChunk * (kAct + 4);
 #pragma unroll
@@ -389,22 +388,25 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
   hi = __uint_as_float(b);
 }
 
-// The scale of a block's sums as (pre, factor): (1, as * ws), or where that
-// product comes near the ends of the range of fp32 (or is not finite) (ws, as),
-// applied one after the other.
-__device__ __forceinline__ float2 split_scale(float as, float ws) {
-  const float f = as * ws;
-  return fabsf(f) >= 0x1p-60f && fabsf(f) <= 0x1p60f ? make_float2(1.f, f) : make_float2(ws, as);
-}
-
-// acc + v * pre * factor; by the lane, so that no row depends on another.
-template <int kCount>
-__device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, float pre, float factor) {
-  if (pre != 1.f) {
-#pragma unroll
-    for (int j = 0; j < kCount; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * pre);
+// acc + v * (as ws).  Where that product comes near the ends of the range of
+// fp32, or is not finite (plain false), the two are applied one after the other;
+// by the lane, so that no row depends on another.
+struct Scale {
+  float factor, pre;
+  bool plain;
+  __device__ __forceinline__ Scale(float as, float ws) : factor(as * ws), pre(ws) {
+    plain = ((__float_as_uint(factor) >> 23) & 255u) - 67u < 120u;  // 2^-60 to 2^60
+    if (!plain) factor = as;
   }
-  const uint64_t ff = pack2(__float_as_uint(factor), __float_as_uint(factor));
+};
+
+template <int kCount>
+__device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, const Scale& s) {
+  if (!s.plain) {
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * s.pre);
+  }
+  const uint64_t ff = pack2(__float_as_uint(s.factor), __float_as_uint(s.factor));
 #pragma unroll
   for (int j = 0; j < kCount / 2; ++j) acc[j] = fma2(pack2(v[2 * j], v[2 * j + 1]), ff, acc[j]);
 }
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         for (int b = 0; b < blocks; ++b, ++g) {
           const int st = (int)(g % P::kStages);
           const uint32_t use = g / P::kStages;
-          if (use > 0 && !tc::mbar_wait(empty(st), (use - 1) & 1u, kWaitLimit)) {
+          if (use > 0 && !tc::mbar_wait_asleep(empty(st), (use - 1) & 1u)) {
             failed = true;
             break;
           }
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       // every stage loaded has been consumed before the CTA may exit
       for (uint32_t u = g > (uint32_t)P::kStages ? g - P::kStages : 0u; u < g; ++u)
-        if (!tc::mbar_wait(empty((int)(u % P::kStages)), (u / P::kStages) & 1u, kWaitLimit)) failed = true;
+        if (!tc::mbar_wait_asleep(empty((int)(u % P::kStages)), (u / P::kStages) & 1u)) failed = true;
     }
     if (warp == kAddWarps + 1 && rank == 0) {  // MMA issuer: the warp waits, one thread issues
       constexpr uint32_t idesc = tc::idesc_e4m3_f32(128 * kCtas, kTileN);
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           // even lanes poll for the operands, odd ones for the TMEM columns: one latency instead of two
           const uint32_t bar = (lane & 1) ? acc_empty(buf) : full(st);
           const uint32_t parity = (lane & 1) ? (buf_use - 1) & 1u : st_use & 1u;
-          const bool ready = ((lane & 1) && buf_use == 0) || tc::mbar_wait(bar, parity, kWaitLimit);
+          const bool ready = ((lane & 1) && buf_use == 0) || tc::mbar_wait_asleep(bar, parity);
           if (!__all_sync(0xffffffffu, ready)) {
             failed = true;
             break;
@@ -603,7 +605,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       // every MMA issued has finished before TMEM is freed
       if (issuer) tc::Ctas<kCtas>::commit(drain);
       __syncwarp();
-      tc::mbar_wait(drain, 0, kWaitLimit);
+      tc::mbar_wait_asleep(drain, 0);
     }
     if (warp >= kAddWarps + 2) {  // scales: thread i copies those of rows i and i + 64, threads 0 and 1 the weights'
       const int i = tid - (kAddWarps + 2) * 32;
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const float *pa0 = as + (live0 ? row0 * as_row : 0), *pa1 = as + (live1 ? (row0 + 64) * as_row : 0);
         const float* pw = ws + (live2 ? half * ws_row : 0);
         for (int b0 = 0; b0 < blocks; b0 += kScaleGroup) {
-          if (use > 0 && !tc::mbar_wait(scale_empty(slot), (use - 1) & 1u, kWaitLimit)) {
+          if (use > 0 && !tc::mbar_wait_asleep(scale_empty(slot), (use - 1) & 1u)) {
             failed = true;
             break;
           }
@@ -641,9 +643,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     uint8_t* buf4k = base + P::kStoreOff + warp * 4096;
     const float* scales = reinterpret_cast<const float*>(base + P::kScaleOff);
     const int my_row = quarter * 32 + lane, my_half = 128 + strip * kCols / kFp8Block;
-    // the issuer's acc_empty[]
-    const uint32_t release0 = tc::map_rank(acc_empty(0), kCtas == 2 ? 0 : part);
-    const uint32_t release1 = tc::map_rank(acc_empty(1), kCtas == 2 ? 0 : part);
+    // Of the block's TMEM buffer, exchanged from block to block: its columns, its
+    // acc_full and the issuer's acc_empty.
+    static_assert(kAccBufs == 2 && kTileN == 256);
+    uint32_t columns = t0, ready = acc_full(0), release = tc::map_rank(acc_empty(0), kCtas == 2 ? 0 : part);
+    const uint32_t other_ready = ready ^ acc_full(1);
+    const uint32_t other_release = release ^ tc::map_rank(acc_empty(1), kCtas == 2 ? 0 : part);
     uint32_t g = 0, gg = 0;
     for (int t = first; t < tiles && !failed; t += step) {
       int mt, nt;
@@ -653,28 +658,27 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = 0;
       for (int b0 = 0; b0 < blocks; b0 += kScaleGroup, ++gg) {
-        if (!failed && !tc::mbar_wait(scale_full(gg % kScaleGroups), (gg / kScaleGroups) & 1u, kWaitLimit)) failed = true;
+        if (!failed && !tc::mbar_wait_asleep(scale_full(gg % kScaleGroups), (gg / kScaleGroups) & 1u)) failed = true;
         const float* slot = scales + gg % kScaleGroups * (kScaleGroup * kScaleBlock / 4);
         const int last = min(blocks - b0, kScaleGroup);
 #pragma unroll 1
         for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock / 4) {
-          const uint32_t buf = g % kAccBufs;
-          if (!failed && !tc::mbar_wait(acc_full(buf), (g / kAccBufs) & 1u, kWaitLimit)) failed = true;
+          if (!failed && !tc::mbar_wait_asleep(ready, (g >> 1) & 1u)) failed = true;
           tc::fence_after_sync();
-          float2 scale;
-#pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            uint32_t v[32];
-            tc::tmem_ld32(t0 + buf * kTileN + c, v);
-            if (c == 0) scale = split_scale(slot[my_row], slot[my_half]);
-            tc::tmem_wait_ld();
-            if (c + 32 == kCols) {
-              tc::fence_before_sync();
-              __syncwarp();
-              if (lane == 0) tc::mbar_arrive_cluster(buf ? release1 : release0);
-            }
-            add_scaled<32>(acc + c / 2, v, scale.x, scale.y);
-          }
+          uint32_t v[32];
+          tc::tmem_ld32(columns, v);
+          const Scale scale(slot[my_row], slot[my_half]);
+          tc::tmem_wait_ld();
+          add_scaled<32>(acc, v, scale);
+          tc::tmem_ld32(columns + 32, v);
+          tc::tmem_wait_ld();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(release);
+          add_scaled<32>(acc + 16, v, scale);
+          columns ^= kTileN;  // TMEM is this CTA's alone: the first buffer starts at column 0
+          ready ^= other_ready;
+          release ^= other_release;
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(scale_empty(gg % kScaleGroups));
