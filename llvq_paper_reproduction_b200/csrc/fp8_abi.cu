@@ -20,6 +20,7 @@ bool on_boundary(const void* p, uintptr_t bytes) { return reinterpret_cast<uintp
 const char* bad_out(const uint8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t cols) {
   if (rows == 0 || cols == 0) return nullptr;
   if (!q || !scale) return "null output";
+  if (rows > llvq::kFp8MaxUnits / ((cols - 1) / llvq::kFp8Block + 1)) return "more than 2^32 - 2^16 blocks";
   if (ldq < cols || ldq % 16 || !on_boundary(q, 16)) return "e4m3 rows must be 16-byte aligned (base and stride)";
   return nullptr;
 }

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (lane == 0) {  // TMA producer
       int i = F::kStages;
       for (; i < count; ++i) {
-        if (!tc::mbar_wait_asleep(empty(i % F::kStages), (i / F::kStages - 1) & 1)) {
+        if (!tc::mbar_wait_for<0>(empty(i % F::kStages), (i / F::kStages - 1) & 1)) {
           failed = true;
           break;
         }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       // no copy may still be in flight when the block exits: wait for the last use of every stage
       i = min(i, count);
       for (int u = i > F::kStages ? i - F::kStages : 0; u < i; ++u)
-        tc::mbar_wait_asleep(full(u % F::kStages), (u / F::kStages) & 1);
+        tc::mbar_wait_for<0>(full(u % F::kStages), (u / F::kStages) & 1);
     }
   } else if (warp == 1) {  // MMA issuer: the warp waits, one thread issues
     constexpr uint32_t idesc = tc::idesc_e4m3_f32(kTileRows, kAct);
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     uint32_t st = 0, st_use = 0;
     for (int i = 0; i < count; ++i) {
       const uint32_t in_group = i % F::kGroup, buf = i / F::kGroup % F::kBufs, use = i / F::kGroup / F::kBufs;
-      if ((in_group == 0 && use > 0 && !tc::mbar_wait_asleep(acc_empty(buf), (use - 1) & 1u)) ||
-          !tc::mbar_wait_asleep(full(st), st_use & 1u)) {
+      if ((in_group == 0 && use > 0 && !tc::mbar_wait_for<0>(acc_empty(buf), (use - 1) & 1u)) ||
+          !tc::mbar_wait_for<0>(full(st), st_use & 1u)) {
         failed = true;
         break;
       }
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // every MMA issued has finished before TMEM is freed
     if (issuer) tc::commit(drain);
     __syncwarp();
-    tc::mbar_wait_asleep(drain, 0);
+    tc::mbar_wait_for<64>(drain, 0);
   } else {  // warps 2..5 read TMEM lane quarters 2, 3, 0, 1
     const int t = tid - 64;
     const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         if (i0 + F::kChunk < count) fetch(i0 / F::kChunk + 1);
       }
       const int buf = i0 / F::kGroup % F::kBufs;
-      if (!failed && !tc::mbar_wait_asleep(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1)) failed = true;
+      if (!failed && !tc::mbar_wait_for<0>(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1)) failed = true;
       tc::fence_after_sync();
       const float* slot = scales + (i0 / F::kChunk & 1) * F::kScaleFloats + i0 % F::kChunk * (kAct + 4);
 #pragma unroll
@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   dependents_may_start();
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
+  __syncwarp();
   tc::cluster_sync();
   if (warp >= 2)
     store_reduced<kTileRows, false>(sbase, rank, splits, y, ldy, y_type, m0, n0, min(kAct, m_total - m0), n_total,
@@ -562,7 +563,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         for (int b = 0; b < blocks; ++b, ++g) {
           const int st = (int)(g % P::kStages);
           const uint32_t use = g / P::kStages;
-          if (use > 0 && !tc::mbar_wait_asleep(empty(st), (use - 1) & 1u)) {
+          if (use > 0 && !tc::mbar_wait_for<64>(empty(st), (use - 1) & 1u)) {
             failed = true;
             break;
           }
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       // every stage loaded has been consumed before the CTA may exit
       for (uint32_t u = g > (uint32_t)P::kStages ? g - P::kStages : 0u; u < g; ++u)
-        if (!tc::mbar_wait_asleep(empty((int)(u % P::kStages)), (u / P::kStages) & 1u)) failed = true;
+        if (!tc::mbar_wait_for<0>(empty((int)(u % P::kStages)), (u / P::kStages) & 1u)) failed = true;
     }
     if (warp == kAddWarps + 1 && rank == 0) {  // MMA issuer: the warp waits, one thread issues
       constexpr uint32_t idesc = tc::idesc_e4m3_f32(128 * kCtas, kTileN);
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           // even lanes poll for the operands, odd ones for the TMEM columns: one latency instead of two
           const uint32_t bar = (lane & 1) ? acc_empty(buf) : full(st);
           const uint32_t parity = (lane & 1) ? (buf_use - 1) & 1u : st_use & 1u;
-          const bool ready = ((lane & 1) && buf_use == 0) || tc::mbar_wait_asleep(bar, parity);
+          const bool ready = ((lane & 1) && buf_use == 0) || tc::mbar_wait_for<0>(bar, parity);
           if (!__all_sync(0xffffffffu, ready)) {
             failed = true;
             break;
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       // every MMA issued has finished before TMEM is freed
       if (issuer) tc::Ctas<kCtas>::commit(drain);
       __syncwarp();
-      tc::mbar_wait_asleep(drain, 0);
+      tc::mbar_wait_for<64>(drain, 0);
     }
     if (warp >= kAddWarps + 2) {  // scales: thread i copies those of rows i and i + 64, threads 0 and 1 the weights'
       const int i = tid - (kAddWarps + 2) * 32;
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const float *pa0 = as + (live0 ? row0 * as_row : 0), *pa1 = as + (live1 ? (row0 + 64) * as_row : 0);
         const float* pw = ws + (live2 ? half * ws_row : 0);
         for (int b0 = 0; b0 < blocks; b0 += kScaleGroup) {
-          if (use > 0 && !tc::mbar_wait_asleep(scale_empty(slot), (use - 1) & 1u)) {
+          if (use > 0 && !tc::mbar_wait_for<256>(scale_empty(slot), (use - 1) & 1u)) {
             failed = true;
             break;
           }
@@ -658,12 +659,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) acc[j] = 0;
       for (int b0 = 0; b0 < blocks; b0 += kScaleGroup, ++gg) {
-        if (!failed && !tc::mbar_wait_asleep(scale_full(gg % kScaleGroups), (gg / kScaleGroups) & 1u)) failed = true;
+        if (!failed && !tc::mbar_wait_for<0>(scale_full(gg % kScaleGroups), (gg / kScaleGroups) & 1u)) failed = true;
         const float* slot = scales + gg % kScaleGroups * (kScaleGroup * kScaleBlock / 4);
         const int last = min(blocks - b0, kScaleGroup);
 #pragma unroll 1
         for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock / 4) {
-          if (!failed && !tc::mbar_wait_asleep(ready, (g >> 1) & 1u)) failed = true;
+          if (!failed && !tc::mbar_wait_for<0>(ready, (g >> 1) & 1u)) failed = true;
           tc::fence_after_sync();
           uint32_t v[32];
           tc::tmem_ld32(columns, v);
@@ -707,6 +708,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   dependents_may_start();
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
+  __syncwarp();
   tc::fence_before_sync();
   tc::cluster_sync();  // partial sums are there; no arrival or commit is under way to a CTA that has left
   tc::fence_after_sync();

@@ -489,7 +489,7 @@ template <typename T, bool kGated, int kStep>
 cudaError_t rows_step(Fp8In x, Fp8In up, int64_t rows, int64_t cols, Fp8Out out, cudaStream_t stream) {
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block, units = rows * blocks;
   constexpr int kTeams = kRowThreads / kGroup, kCta = kTeams * kRowUnits<T, kGated>;
-  if (units > 0xFFFFFFFFLL - kCta) return cudaErrorInvalidValue;
+  if (units > kFp8MaxUnits) return cudaErrorInvalidValue;
   return launch_overlapped(rows_kernel<T, kGated, kStep>, dim3((unsigned)((units + kCta - 1) / kCta)), kRowThreads, 0, 0,
                            stream, static_cast<const T*>(x.ptr), x.ld, static_cast<const T*>(up.ptr), up.ld,
                            (uint32_t)rows, (uint32_t)blocks, (uint32_t)(kTeams / blocks), (uint32_t)(kTeams % blocks),
@@ -593,7 +593,7 @@ cudaError_t fp8_rms_norm_launch(Fp8In x, Fp8In residual, int type, const void* w
                                 int64_t rows, int64_t cols, void* hidden, int64_t ld_hidden, Fp8Out out,
                                 cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return cudaSuccess;
-  if (cols > kFp8NormMaxCols || rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  if (cols > kFp8NormMaxCols) return cudaErrorInvalidValue;
   const NormCall n{x, residual, weight, eps, rows, cols, hidden, ld_hidden, out, stream};
   if (type == LLVQ_DT_F32) return norm_typed<float, float>(n);
   if (type == LLVQ_DT_F16)

@@ -164,6 +164,7 @@ cudaError_t hadamard_launch(const void* in, int in_type, void* out, int out_type
 // 8-bit operators (fp8_quant.cu, fp8_gemm.cu): e4m3 values with one fp32
 // scale per block of 128 columns.  Element types: LLVQ_DT_*.
 constexpr int kFp8Block = 128;
+constexpr int64_t kFp8MaxUnits = 0xFFFF0000LL;  // (row, block) pairs of a quantizer call: they are numbered in 32 bits
 constexpr int64_t kFp8NormMaxCols = 32768;  // a row of the norm stays in the registers of one CTA
 
 // Where a quantizer writes: e4m3 rows (row stride ld, a multiple of 16, base

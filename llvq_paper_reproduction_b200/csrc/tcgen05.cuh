@@ -124,26 +124,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 
 // ---- 8-bit operands and clusters (fp8_gemm.cu)
 
-// Wait for phase `parity` of an mbarrier, giving up after about two seconds.
-// Each poll may sleep (the hint, in ns) until the phase ends: warps that wait
-// for long take no issue slots from those that work.
-__device__ __forceinline__ bool mbar_try(uint32_t mbar_saddr, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(mbar_saddr), "r"(parity), "r"(1000000)
-      : "memory");
-  return done != 0;
-}
-
-__device__ __forceinline__ bool mbar_wait_asleep(uint32_t mbar_saddr, uint32_t parity) {
-  if (mbar_try(mbar_saddr, parity)) return true;
-  const long long begin = clock64();
-  do {
-    if (mbar_try(mbar_saddr, parity)) return true;
-  } while (clock64() - begin < 4000000000LL);
+// mbar_wait with kSleep nanoseconds between polls, for warps whose polls would
+// take issue slots from those that work and that need not know at once.
+template <int kSleep>
+__device__ __forceinline__ bool mbar_wait_for(uint32_t mbar_saddr, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    if (mbar_wait(mbar_saddr, parity, 1)) return true;
+    if (kSleep) __nanosleep(kSleep);
+  }
   return false;
 }
 

@@ -54,6 +54,7 @@ P = 1 << 20  # an address that is never read: every call below is refused first
     lambda: _native.fp8_quantize(P, 0, 128, 2, 128, 1, P, 120, P, 1, 1, 0),        # e4m3 stride below the columns
     lambda: _native.fp8_quantize(0, 0, 128, 1, 128, 1, P, 128, P, 1, 1, 0),        # null input
     lambda: _native.fp8_quantize(P, 0, 128, 1, 128, 1, P, 128, 0, 1, 1, 0),        # null scale
+    lambda: _native.fp8_quantize(P, 0, 1, 1 << 32, 1, 1, P, 16, P, 1, 1, 0),       # too many blocks
     lambda: _native.fp8_swiglu(P, 128, 0, 128, 0, 1, 128, P, 128, P, 1, 1, 0),     # null up
     lambda: _native.fp8_swiglu(P, 128, P, 128, 7, 1, 128, P, 128, P, 1, 1, 0),     # unknown type
     lambda: _native.fp8_rms_norm(P, 128, 0, 0, 1, P, 2, 1e-5, 1, 128, 0, 0, P, 128, P, 1, 1, 0),  # weight's type

@@ -107,6 +107,21 @@ def test_quantizer_strides_and_empty(dtype):
         assert q.shape == shape and scale.shape == ((shape[0] + 127) // 128, (shape[1] + 127) // 128)
 
 
+def test_more_than_2_to_the_31_rows():
+    """Rows are counted past 31 bits too: 2.2e9 rows of one column."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    m = (1 << 31) + 70_000
+    x = torch.zeros((m, 1), dtype=torch.bfloat16, device="cuda")
+    x[-2:] = torch.tensor([[3.0], [-5.0]], device="cuda")
+    q, scale = fp8.quantize_rows(x)
+    assert q[-2:].float().flatten().tolist() == [448.0, -448.0] and not q[:1000].float().any()
+    assert (scale[-2:].flatten() * 448 - torch.tensor([3.0, 5.0], device="cuda")).abs().max() < 1e-5
+    del q, scale
+    q, scale = fp8.rms_norm(x, torch.ones(1, dtype=torch.bfloat16, device="cuda"))
+    assert q[-2:].float().flatten().tolist() == [448.0, -448.0]
+
+
 def test_quantizer_past_32_bit_offsets():
     from llvq_paper_reproduction_b200 import fp8
 
@@ -392,6 +407,48 @@ def test_mlp_captured_and_on_another_stream(m):
     assert torch.equal(want, other)
     for _, out in graphs:
         assert torch.equal(out[0], want2) and torch.equal(out[1], hidden2)
+
+
+FIRST_CALLS = """
+import torch
+from llvq_paper_reproduction_b200 import fp8
+x = torch.randn(600, 520, device="cuda").to(torch.bfloat16)
+w = torch.ones(520, device="cuda", dtype=torch.bfloat16)
+a, b = fp8.quantize_rows(x[:1]), fp8.quantize_blocks(x)
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        fp8.gemm(*a, *b)
+except RuntimeError as e:
+    assert "before capturing" in str(e), e
+else:
+    raise AssertionError("the error flag would have been taken from the graph's memory")
+torch.cuda.synchronize()
+fp8.gemm(*a, *b)  # one size only: the other kernels are first called in the capture
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q, s, h = fp8.rms_norm(x, w, residual=x)
+    y = fp8.gemm(q, s, *b)
+    z = fp8.swiglu(y, y)
+g.replay()
+torch.cuda.synchronize()
+q2, s2, h2 = fp8.rms_norm(x, w, residual=x)
+y2 = fp8.gemm(q2, s2, *b)
+assert torch.equal(y, y2) and torch.equal(h, h2) and y.isfinite().all()
+assert torch.equal(z[0].float(), fp8.swiglu(y2, y2)[0].float())
+print("fine")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process: kernels whose first call is captured, and the
+    product's demand for one call before."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "fine", done.stderr[-2000:]
 
 
 def test_calls_do_not_synchronise_the_host():
