@@ -17,7 +17,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <cstring>
 #include <type_traits>
 
 #include "fp8_launch.cuh"
@@ -337,19 +336,25 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 // K blocks are split over a cluster, which adds its partial sums through
 // distributed shared memory in rank order.
 //
-// Roles: warps 0..15 add up (lane quarter warp % 4, column quarter warp / 4),
-// warp 16 loads with TMA, warp 17 (of the leading CTA) issues the MMAs, warps
-// 18 and 19 bring the scales, kScaleGroup blocks at a time and two groups in
-// flight.  Adding is a chain of waits (block sum ready, TMEM load, hand back),
-// so it takes four warps per scheduler to keep up with the tensor cores: with
-// two, of twice the columns, a block took 1300 cycles for the 512 of its MMAs.
-// TMEM holds two block sums of 256 columns.  In a pair the leader's full[]
-// takes the bytes of both CTAs' loads; empty[] and acc_full[] are committed in
-// both CTAs; the leader's acc_empty[] takes the arrivals of all 32 adding warps.
-constexpr int kAddWarps = 16;
+// Roles: warps 0..7 add up (lane quarter warp % 4, column half warp / 4), warp 8
+// loads with TMA, warp 9 (of the leading CTA) issues the MMAs, warps 10 and 11
+// bring the scales, kScaleGroup blocks at a time and two groups in flight.  TMEM
+// holds two block sums of 256 columns.  In a pair the leader's full[] takes the
+// bytes of both CTAs' loads; empty[] and acc_full[] are committed in both CTAs;
+// the leader's acc_empty[] takes the arrivals of all 16 adding warps.
+//
+// What bounds it: a block costs about 860 cycles where its MMAs take 512
+// (4096 x 14336 x 4096: 219 us, 2.2 PFLOP/s; without the additions 191, without
+// the TMEM loads too 176).  An adding warp's pass is a chain of latencies: the
+// block's sums ready, a TMEM load, 32 FFMA2, a second load, the buffer handed
+// back, 32 FFMA2 (2.4 cycles each on a scheduler); hence loads of 64 columns, and
+// the look for the next block before the last additions.  Measured beside it:
+// 16 warps of 64 columns at 112 registers 225 us; halves of the buffer handed
+// back apart 237; tiles of 192 columns read in one piece 262.
+constexpr int kAddWarps = 8;
 constexpr int kWideThreads = kAddWarps * 32 + 128;
-// 640 threads launch with 96 registers each: 61,440 = 512 x 112 + 128 x 32
-constexpr int kAddRegs = 112, kOtherRegs = 32;
+// 384 threads launch with 168 registers each: 64,512 = 256 x 224 + 128 x 56
+constexpr int kAddRegs = 224, kOtherRegs = 56;
 constexpr int kTileN = 256;
 constexpr int kCols = kTileN / (kAddWarps / 4);  // columns of an adding warp
 constexpr int kAccBufs = 512 / kTileN;
@@ -360,7 +365,7 @@ template <int kCtas>
 struct Wide {
   static constexpr int kStageA = 128 * 128, kStageB = kTileN / kCtas * 128;
   static constexpr int kStageBytes = kStageA + kStageB;
-  static constexpr int kStages = 4;
+  static constexpr int kStages = kCtas == 2 ? 5 : 4;
   // 4 KB per adding warp to store through; a CTA with a single tile stores when its stages are free
   static constexpr int kStoreOff = kCtas == 2 ? kStages * kStageBytes : 0;
   static constexpr int kScaleOff = kCtas == 2 ? kStoreOff + kAddWarps * 4096 : kStages * kStageBytes;
@@ -413,15 +418,20 @@ __device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, const Sca
 }
 
 // A warp's 32 rows x kWidth columns to y, through its 4 KB of shared memory (32
-// rows of 128 bytes, 16-byte chunks swizzled by the row) so that the global
-// stores are whole 128-byte lines.
+// rows of 128 bytes in the 128-byte swizzle).  Where y's rows start on 16-byte
+// boundaries (tma) the buffer leaves by an asynchronous TMA store, clipped at
+// the matrix's ends; else a row of it at a time, four bytes a lane.
 template <typename T, int kWidth>
-__device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0,
-                                           int col0, int m_total, int n_total, int lane) {
+__device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, const CUtensorMap* ty, bool tma,
+                                           T* __restrict__ y, int64_t ldy, int row0, int col0, int m_total, int n_total,
+                                           int lane) {
   constexpr int kPerLine = 128 / (int)sizeof(T), kPerChunk = 16 / (int)sizeof(T);
-  const bool whole = ldy * (int64_t)sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
 #pragma unroll
   for (int c0 = 0; c0 < kWidth; c0 += kPerLine) {
+    if (tma) {
+      if (lane == 0) tc::bulk_wait_read();  // the store before has read the buffer
+      __syncwarp();
+    }
 #pragma unroll
     for (int ch = 0; ch < 8; ++ch) {
       alignas(16) T e[kPerChunk];
@@ -434,33 +444,20 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T*
       }
       *reinterpret_cast<uint4*>(buf + lane * 128 + ((ch ^ (lane & 7)) * 16)) = *reinterpret_cast<const uint4*>(e);
     }
-    __syncwarp();
-    if (whole) {
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int r = it * 4 + (lane >> 3), ch = lane & 7;
-        const int row = row0 + r, col = col0 + c0 + ch * kPerChunk;
-        const uint4 v = *reinterpret_cast<const uint4*>(buf + r * 128 + ((ch ^ (r & 7)) * 16));
-        if (row < m_total && col < n_total) {  // 
-          T* dst = y + (int64_t)row * ldy + col;
-          if (col + kPerChunk <= n_total) {
-            *reinterpret_cast<uint4*>(dst) = v;
-          } else {
-            const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int j = 0; j < kPerChunk; ++j)
-              if (col + j < n_total) dst[j] = e[j];
-          }
-        }
-      }
-    } else {  // rows off 16-byte boundaries: a row of the buffer at a time, four bytes a lane
+    if (tma) {
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0 && row0 < m_total && col0 + c0 < n_total) tc::tma_store_2d(ty, col0 + c0, row0, tc::smem_addr(buf));
+    } else {
+      __syncwarp();
       constexpr int kPerWord = 4 / (int)sizeof(T);
       const int col = col0 + c0 + lane * kPerWord;
       const bool words = ldy * (int64_t)sizeof(T) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0;
 #pragma unroll 4
       for (int r = 0; r < 32; ++r) {
         if (row0 + r >= m_total || col >= n_total) break;
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+        const uint32_t v =
+            *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
         T* dst = y + (int64_t)(row0 + r) * ldy + col;
         if (words && col + kPerWord <= n_total) {
           *reinterpret_cast<uint32_t*>(dst) = v;
@@ -470,8 +467,8 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, T*
           if (kPerWord > 1 && col + 1 < n_total) dst[kPerWord - 1] = e[kPerWord - 1];
         }
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -488,7 +485,8 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& mt, int& nt)
 // tile per cluster of `split` CTAs.
 template <int kCtas>
 __global__ void __launch_bounds__(kWideThreads, 1)
-    wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tw, int blocks_total,
+    wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tw,
+                const __grid_constant__ CUtensorMap ty, bool tma_store, int blocks_total,
                 const float* __restrict__ as, int64_t as_row, int64_t as_col, const float* __restrict__ ws,
                 int64_t ws_row, int64_t ws_col, int m_total, int n_total, void* __restrict__ y, int64_t ldy, int y_type,
                 int tm, int tn, int splits, int* error_flag) {
@@ -650,7 +648,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     uint32_t columns = t0, ready = acc_full(0), release = tc::map_rank(acc_empty(0), kCtas == 2 ? 0 : part);
     const uint32_t other_ready = ready ^ acc_full(1);
     const uint32_t other_release = release ^ tc::map_rank(acc_empty(1), kCtas == 2 ? 0 : part);
-    uint32_t g = 0, gg = 0;
+    uint32_t g = 0, gg = 0, seen = 0;  // seen: block g's sums are known to be there
     for (int t = first; t < tiles && !failed; t += step) {
       int mt, nt;
       tile_at(t, tm, tn, mt, nt);
@@ -664,22 +662,23 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const int last = min(blocks - b0, kScaleGroup);
 #pragma unroll 1
         for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock / 4) {
-          if (!failed && !tc::mbar_wait_for<0>(ready, (g >> 1) & 1u)) failed = true;
+          if (!seen && !failed && !tc::mbar_wait_for<0>(ready, (g >> 1) & 1u)) failed = true;
           tc::fence_after_sync();
-          uint32_t v[32];
-          tc::tmem_ld32(columns, v);
+          uint32_t v[64];
+          tc::tmem_ld64(columns, v);
           const Scale scale(slot[my_row], slot[my_half]);
           tc::tmem_wait_ld();
-          add_scaled<32>(acc, v, scale);
-          tc::tmem_ld32(columns + 32, v);
+          add_scaled<64>(acc, v, scale);
+          tc::tmem_ld64(columns + 64, v);
           tc::tmem_wait_ld();
           tc::fence_before_sync();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_cluster(release);
-          add_scaled<32>(acc + 16, v, scale);
           columns ^= kTileN;  // TMEM is this CTA's alone: the first buffer starts at column 0
           ready ^= other_ready;
           release ^= other_release;
+          seen = tc::mbar_peek(ready, ((g + 1) >> 1) & 1u);
+          add_scaled<64>(acc + 32, v, scale);
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(scale_empty(gg % kScaleGroups));
@@ -694,15 +693,18 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           tc::st_shared4(partial_at<kTileN, true>(sbase, my_row, strip * (kCols / 4) + j), x, y_, z, w);
         }
       } else if (y_type == LLVQ_DT_F32) {
-        store_rows<float, kCols>(acc, buf4k, static_cast<float*>(y), ldy, row0, col0, m_total, n_total, lane);
+        store_rows<float, kCols>(acc, buf4k, &ty, tma_store, static_cast<float*>(y), ldy, row0, col0, m_total, n_total,
+                                 lane);
       } else if (y_type == LLVQ_DT_F16) {
-        store_rows<__half, kCols>(acc, buf4k, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total, lane);
+        store_rows<__half, kCols>(acc, buf4k, &ty, tma_store, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total,
+                                  lane);
       } else {
-        store_rows<__nv_bfloat16, kCols>(acc, buf4k, static_cast<__nv_bfloat16*>(y), ldy, row0, col0, m_total, n_total,
-                                         lane);
+        store_rows<__nv_bfloat16, kCols>(acc, buf4k, &ty, tma_store, static_cast<__nv_bfloat16*>(y), ldy, row0, col0,
+                                         m_total, n_total, lane);
       }
     }
   }
+  if (warp < kAddWarps && lane == 0) tc::bulk_wait();  // y is written before the kernel ends
   // not earlier: CTAs of the next product placed two on one of the idle SMs would share it to their end
   // (64 x 4096 x 14336: 20.5 us against 17.1)
   dependents_may_start();
@@ -737,6 +739,21 @@ cudaError_t encode_e4m3_map(CUtensorMap* map, const void* ptr, int64_t cols, int
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// y [rows, cols] of LLVQ_DT_* type (row stride ld elements), box 32 rows x 128 bytes, 128-byte swizzle.
+cudaError_t encode_out_map(CUtensorMap* map, void* ptr, int64_t cols, int64_t rows, int64_t ld, int type) {
+  const auto enc = tensor_map_encoder();
+  if (!enc) return cudaErrorNotSupported;
+  const int size = type == LLVQ_DT_F32 ? 4 : 2;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = enc(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, ptr, dims,
+                         strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
@@ -843,16 +860,22 @@ cudaError_t wide_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int n, 
                         int y_type, int* error_flag, int sms, int splits, cudaStream_t stream) {
   cudaError_t e = configure_wide<kCtas>();
   if (e != cudaSuccess) return e;
-  CUtensorMap ta, tw;
+  CUtensorMap ta, tw, ty = {};
   e = encode_e4m3_map(&ta, a.q, k, m, a.ld, 128);
   if (e != cudaSuccess) return e;
   e = encode_e4m3_map(&tw, w.q, k, n, w.ld, kTileN / kCtas);
   if (e != cudaSuccess) return e;
   const int64_t tm = (m + 128LL * kCtas - 1) / (128 * kCtas), tn = (n + (int64_t)kTileN - 1) / kTileN;
   if (tm * tn > (1 << 27)) return cudaErrorInvalidValue;
+  const int size = y_type == LLVQ_DT_F32 ? 4 : 2;
+  const bool tma_store = ldy * size % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  if (tma_store) {
+    e = encode_out_map(&ty, y, n, m, ldy, y_type);
+    if (e != cudaSuccess) return e;
+  }
   const int64_t grid = kCtas == 2 ? 2 * std::min<int64_t>(tm * tn, sms / 2) : tm * tn * splits;
   return launch_overlapped(wide_kernel<kCtas>, dim3((unsigned)grid), kWideThreads, Wide<kCtas>::kSmem,
-                           kCtas == 2 ? 2 : splits, stream, ta, tw, (k + kFp8Block - 1) / kFp8Block, a.scale,
+                           kCtas == 2 ? 2 : splits, stream, ta, tw, ty, tma_store, (k + kFp8Block - 1) / kFp8Block, a.scale,
                            a.scale_row, a.scale_col, w.scale, w.scale_row, w.scale_col, m, n, y, ldy, y_type, (int)tm,
                            (int)tn, splits, error_flag);
 }
