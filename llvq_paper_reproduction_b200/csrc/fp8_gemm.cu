@@ -39,6 +39,32 @@ __device__ __forceinline__ T to_out(float v) {
   else return __float2bfloat16_rn(v);
 }
 
+// Two fp32 values in a register pair.
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+
 // Four neighbouring outputs, `count` of them in the matrix; whole: 16-byte stores are possible.
 __device__ __forceinline__ void store4(void* y, int64_t i, float4 v, int type, bool whole, int count) {
   if (type == LLVQ_DT_F32) {
@@ -142,7 +168,7 @@ struct Few {
   static constexpr int kBarOff = kScaleOff + 2 * kScaleFloats * 4;
   static constexpr int kBars = 2 * kStages + 2 * kBufs + 1;
   static constexpr size_t kSmem = (size_t)kBarOff + 8 * kBars + 16 + 1024;
-  static_assert(kStages >= 2 && kAct * kTileRows * 4 <= kScaleOff && kScaleOff % 16 == 0 && kBarOff % 8 == 0);
+  static_assert(kAct * kGroup == 64 && kStages >= 2 && kAct * kTileRows * 4 <= kScaleOff && kScaleOff % 16 == 0 && kBarOff % 8 == 0);
   static_assert(kSmem > 76 * 1024 && kSmem <= 113 * 1024);
 };
 
@@ -200,7 +226,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   tc::fence_after_sync();
   const uint32_t tmem = *holder;
   bool failed = false;
-  float acc[kAct];
+  uint64_t acc[kAct / 2];
   wait_for_inputs();
 
   if (warp == 0) {
@@ -265,7 +291,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       tc::cp_async_commit();
     };
 #pragma unroll
-    for (int j = 0; j < kAct; ++j) acc[j] = 0.f;
+    for (int j = 0; j < kAct / 2; ++j) acc[j] = 0;
+    uint32_t seen = 0;  // the next group's sums are known to be there
     fetch(0);
     for (int i0 = 0; i0 < count; i0 += F::kGroup) {
       if (i0 % F::kChunk == 0) {
@@ -273,29 +300,31 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         asm volatile("bar.sync 1, 128;" ::: "memory");  // this chunk is whole, and nobody reads the last one any more
         if (i0 + F::kChunk < count) fetch(i0 / F::kChunk + 1);
       }
-      const int buf = i0 / F::kGroup % F::kBufs;
-      if (!failed && !tc::mbar_wait_for<0>(acc_full(buf), (i0 / F::kGroup / F::kBufs) & 1)) failed = true;
+      const int g = i0 / F::kGroup, buf = g % F::kBufs;
+      if (!seen && !failed && !tc::mbar_wait_for<0>(acc_full(buf), (g / F::kBufs) & 1)) failed = true;
       tc::fence_after_sync();
-      const float* slot = scales + (i0 / F::kChunk & 1) * F::kScaleFloats + i0 % F::kChunk * (kAct + 4);
+      uint32_t v[64];
+      tc::tmem_ld64(t0 + buf * 64, v);
+      const uint32_t slot =
+          tc::smem_addr(scales) + ((i0 / F::kChunk & 1) * F::kScaleFloats + i0 % F::kChunk * (kAct + 4)) * 4;
+      tc::tmem_wait_ld();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(acc_empty(buf));
+      seen = tc::mbar_peek(acc_full((g + 1) % F::kBufs), ((g + 1) / F::kBufs) & 1);
 #pragma unroll
-      for (int c = 0; c < F::kGroup * kAct; c += 32) {
-        uint32_t v[32];
-        tc::tmem_ld32(t0 + buf * (F::kGroup * kAct) + c, v);
-        tc::tmem_wait_ld();
-        if (c + 32 == F::kGroup * kAct) {
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(acc_empty(buf));
-        }
+      for (int u = 0; u < F::kGroup; ++u) {
+        if (i0 + u < count) {
+          const uint32_t row = slot + u * (kAct + 4) * 4;
+          const uint32_t w = tc::ld_shared_bits(row + kAct * 4);
+          const uint64_t ww = pack2(w, w);
 #pragma unroll
-        for (int q = 0; q < 32; q += 16) {
-          const int u = (c + q) / kAct, j0 = (c + q) % kAct;
-          if (i0 + u < count) {
-            const float* row = slot + u * (kAct + 4);
-            const float w = row[kAct];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              acc[j0 + j] = fmaf(__uint_as_float(v[q + j]) * w, row[j0 + j], acc[j0 + j]);
+          for (int j = 0; j < kAct; j += 4) {  // the weight's scale, then the row's: their product may leave fp32's range
+            uint64_t s0, s1;
+            tc::ld_shared_pairs(row + j * 4, s0, s1);
+            const uint32_t* x = v + u * kAct + j;
+            acc[j / 2] = fma2(mul2(pack2(x[0], x[1]), ww), s0, acc[j / 2]);
+            acc[j / 2 + 1] = fma2(mul2(pack2(x[2], x[3]), ww), s1, acc[j / 2 + 1]);
           }
         }
       }
@@ -303,7 +332,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     // the last block's sums have been read, so every stage has been consumed: reuse them
     float* part = reinterpret_cast<float*>(base) + (warp & 3) * 32 + lane;
 #pragma unroll
-    for (int j = 0; j < kAct; ++j) part[j * kTileRows] = acc[j];
+    for (int j = 0; j < kAct; j += 2) unpack2(acc[j / 2], part[j * kTileRows], part[(j + 1) * kTileRows]);
   }
   // not earlier: CTAs of the next product placed two on one of the idle SMs would share it to their end
   // (64 x 4096 x 14336: 20.5 us against 17.1)
@@ -374,25 +403,6 @@ struct Wide {
   static constexpr size_t kSmem = (size_t)kBarOff + 8 * kBars + 16 + 1024;
   static_assert(kSmem <= 227 * 1024 && kScaleOff >= 128 * kTileN * 4);
 };
-
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
-}
 
 // acc + v * (as ws).  Where that product comes near the ends of the range of
 // fp32, or is not finite (plain false), the two are applied one after the other;

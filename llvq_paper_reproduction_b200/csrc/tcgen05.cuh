@@ -230,6 +230,17 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t ld_shared_bits(uint32_t saddr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(saddr) : "memory");
+  return v;
+}
+
+// Four fp32 values as two register pairs.
+__device__ __forceinline__ void ld_shared_pairs(uint32_t saddr, uint64_t& a, uint64_t& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(saddr) : "memory");
+}
+
 // Asynchronous 4-byte copy into shared memory, zero when `live` is false.
 __device__ __forceinline__ void cp_async4(uint32_t saddr, const void* p, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(saddr), "l"(p), "r"(live ? 4 : 0) : "memory");
