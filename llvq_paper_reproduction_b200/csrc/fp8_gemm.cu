@@ -779,13 +779,15 @@ cudaError_t configure_once(const void* kernel, size_t smem, std::atomic<bool>* d
   return e;
 }
 
-// CTAs per tile: one CTA per SM where a number of them comes near that (32
-// tiles: 4; 16: 8), else as many as fit two per SM (86 tiles: 3).  4096 x 4096 at
-// m = 1: 4 CTAs a tile 6.8 us, 8 7.4; 11008 x 4096: 3 CTAs 11.4, 1 12.8.
+// CTAs per tile: one CTA per SM where a number of them comes near that and
+// leaves each fewer than 16 blocks (32 tiles of 32 blocks: 4; 16 tiles: 8), else
+// as many as fit two per SM (86 tiles: 3; 32 tiles of 112 blocks: 8).  At m = 1,
+// 4096 x 4096: 4 CTAs a tile 5.7 us, 8 6.2; 4096 x 14336: 4 13.0, 8 11.7; 11008
+// x 4096: 3 CTAs 9.6, 1 11.9.
 int few_splits(int64_t tiles, int64_t blocks, int sms) {
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>({2 * sms / tiles, kMaxSplits, blocks}));
   const int64_t one_each = std::min(sms / tiles, most);
-  return (int)(one_each > 0 && one_each * tiles * 20 >= 17 * sms ? one_each : most);
+  return (int)(one_each > 0 && one_each * tiles * 20 >= 17 * sms && blocks < 16 * one_each ? one_each : most);
 }
 
 template <int kAct>
@@ -912,14 +914,15 @@ cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, in
   int64_t cycles = 0;
   e = choose_splits(tiles, blocks, &splits, &cycles);
   if (e != cudaSuccess) return e;
-  // Tiles of 64 activation rows take 7500 cycles and 800 a block while the SMs
-  // hold one CTA each: shorter where the wide tiles would be few and their parts
-  // many.  128 x 4096 x 4096: 11.6 us against 14.1; 128 x 4096 x 14336: 26.8
-  // against 21.1; 512 x 1024 x 4096: 11.4 against 13.4.
+  // Tiles of 64 activation rows take 7500 cycles and 650 a block while the SMs
+  // hold one CTA each (1000 with two): shorter where the wide tiles would be few
+  // and their parts many.  128 x 4096 x 4096: 10.7 us against 14.1; 128 x 4096 x
+  // 14336: 26.8 against 19.9; 512 x 1024 x 4096: 11.4 against 13.4.
   const int64_t few = (m + 63) / 64 * ((n + kTileRows - 1) / kTileRows);
   if (2 * few <= sms) {
     const int s = few_splits(few, blocks, sms);
-    if (7500 + 800 * ((blocks + s - 1) / s) < cycles) return few_rows_launch<64>(LLVQ_CALL, stream);
+    if (7500 + (s * few <= sms ? 650 : 1000) * ((blocks + s - 1) / s) < cycles)
+      return few_rows_launch<64>(LLVQ_CALL, stream);
   }
   return wide_launch<1>(LLVQ_CALL, splits, stream);
 #undef LLVQ_CALL
