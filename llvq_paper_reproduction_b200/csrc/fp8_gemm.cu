@@ -427,10 +427,36 @@ __device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, const Sca
   for (int j = 0; j < kCount / 2; ++j) acc[j] = fma2(pack2(v[2 * j], v[2 * j + 1]), ff, acc[j]);
 }
 
+// The buffer of store_rows by stores of sizeof(U) bytes, on whose boundaries y's rows start.
+template <typename T, typename U>
+__device__ __forceinline__ void store_lines(const uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0, int col0,
+                                            int m_total, int n_total, int lane) {
+  constexpr int kPer = (int)(sizeof(U) / sizeof(T)), kLanes = 128 / (int)sizeof(U);  // lanes a row, 64 for 2 bytes
+  constexpr int kRows = kLanes < 32 ? 32 / kLanes : 1;
+#pragma unroll 4
+  for (int r = kLanes < 32 ? lane / kLanes : 0; r < 32; r += kRows) {
+#pragma unroll
+    for (int l = lane % kLanes; l < kLanes; l += 32) {
+      const int byte = l * (int)sizeof(U), col = col0 + l * kPer;
+      if (row0 + r >= m_total || col >= n_total) continue;
+      const U v = *reinterpret_cast<const U*>(buf + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15));
+      T* dst = y + (int64_t)(row0 + r) * ldy + col;
+      if (col + kPer <= n_total) {
+        *reinterpret_cast<U*>(dst) = v;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (col + j < n_total) dst[j] = e[j];
+      }
+    }
+  }
+}
+
 // A warp's 32 rows x kWidth columns to y, through its 4 KB of shared memory (32
 // rows of 128 bytes in the 128-byte swizzle).  Where y's rows start on 16-byte
 // boundaries (tma) the buffer leaves by an asynchronous TMA store, clipped at
-// the matrix's ends; else a row of it at a time, four bytes a lane.
+// the matrix's ends; else by stores of 8, 4 or 2 bytes a lane.
 template <typename T, int kWidth>
 __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, const CUtensorMap* ty, bool tma,
                                            T* __restrict__ y, int64_t ldy, int row0, int col0, int m_total, int n_total,
@@ -460,23 +486,10 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, co
       if (lane == 0 && row0 < m_total && col0 + c0 < n_total) tc::tma_store_2d(ty, col0 + c0, row0, tc::smem_addr(buf));
     } else {
       __syncwarp();
-      constexpr int kPerWord = 4 / (int)sizeof(T);
-      const int col = col0 + c0 + lane * kPerWord;
-      const bool words = ldy * (int64_t)sizeof(T) % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0;
-#pragma unroll 4
-      for (int r = 0; r < 32; ++r) {
-        if (row0 + r >= m_total || col >= n_total) break;
-        const uint32_t v =
-            *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
-        T* dst = y + (int64_t)(row0 + r) * ldy + col;
-        if (words && col + kPerWord <= n_total) {
-          *reinterpret_cast<uint32_t*>(dst) = v;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&v);
-          dst[0] = e[0];
-          if (kPerWord > 1 && col + 1 < n_total) dst[kPerWord - 1] = e[kPerWord - 1];
-        }
-      }
+      const uintptr_t at = reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * (int64_t)sizeof(T));
+      if (at % 8 == 0) store_lines<T, uint2>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
+      else if (at % 4 == 0) store_lines<T, uint32_t>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
+      else store_lines<T, T>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
       __syncwarp();
     }
   }
@@ -622,10 +635,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       for (int t = first; t < tiles && !failed; t += step) {
         int mt, nt;
         tile_at(t, tm, tn, mt, nt);
-        const int row0 = (mt * kCtas + rank) * 128 + i, half = nt * (kTileN / kFp8Block) + i;
-        const bool live0 = row0 < m_total, live1 = row0 + 64 < m_total, live2 = half * kFp8Block < n_total;
-        const float *pa0 = as + (live0 ? row0 * as_row : 0), *pa1 = as + (live1 ? (row0 + 64) * as_row : 0);
-        const float* pw = ws + (live2 ? half * ws_row : 0);
+        // rows past the last take the last one's scale, not zero: zero is outside the plain range, and a tile
+        // that is not full would run the additions' other branch (400 x 14336 x 4096: 42 us against 35)
+        const int row0 = (mt * kCtas + rank) * 128 + i, last_row = m_total - 1;
+        const int half = min(nt * (kTileN / kFp8Block) + i, (n_total - 1) / kFp8Block);
+        const float *pa0 = as + min(row0, last_row) * as_row, *pa1 = as + min(row0 + 64, last_row) * as_row;
+        const float* pw = ws + half * ws_row;
         for (int b0 = 0; b0 < blocks; b0 += kScaleGroup) {
           if (use > 0 && !tc::mbar_wait_for<256>(scale_empty(slot), (use - 1) & 1u)) {
             failed = true;
@@ -634,9 +649,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           uint32_t dst = sbase + P::kScaleOff + slot * (kScaleGroup * kScaleBlock) + i * 4;
           const int last = min(b0 + kScaleGroup, blocks);
           for (int b = b_begin + b0; b < b_begin + last; ++b, dst += kScaleBlock) {
-            tc::cp_async4(dst, pa0 + b * as_col, live0);
-            tc::cp_async4(dst + 256, pa1 + b * as_col, live1);
-            if (i < 2) tc::cp_async4(dst + 512, pw + b * ws_col, live2);
+            tc::cp_async4(dst, pa0 + b * as_col, true);
+            tc::cp_async4(dst + 256, pa1 + b * as_col, true);
+            if (i < 2) tc::cp_async4(dst + 512, pw + b * ws_col, true);
           }
           tc::cp_async_arrive(scale_full(slot));
           if (++slot == kScaleGroups) slot = 0, ++use;
@@ -779,15 +794,22 @@ cudaError_t configure_once(const void* kernel, size_t smem, std::atomic<bool>* d
   return e;
 }
 
-// CTAs per tile: one CTA per SM where a number of them comes near that and
-// leaves each fewer than 16 blocks (32 tiles of 32 blocks: 4; 16 tiles: 8), else
-// as many as fit two per SM (86 tiles: 3; 32 tiles of 112 blocks: 8).  At m = 1,
-// 4096 x 4096: 4 CTAs a tile 5.7 us, 8 6.2; 4096 x 14336: 4 13.0, 8 11.7; 11008
-// x 4096: 3 CTAs 9.6, 1 11.9.
-int few_splits(int64_t tiles, int64_t blocks, int sms) {
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({2 * sms / tiles, kMaxSplits, blocks}));
-  const int64_t one_each = std::min(sms / tiles, most);
-  return (int)(one_each > 0 && one_each * tiles * 20 >= 17 * sms && blocks < 16 * one_each ? one_each : most);
+// CTAs per tile, in one wave, by the cycles measured for a CTA: 650 a block
+// while an SM holds one, 1000 and 2500 more where it holds two; 7500 to start, add
+// the parts and store.  At m = 1, 4096 x 4096: 4 CTAs a tile 5.7 us, 8 6.2; 4096 x
+// 14336: 4 13.0, 8 11.7; 11008 x 4096: 3 CTAs 9.6, 1 11.9.
+int few_splits(int64_t tiles, int64_t blocks, int sms, int64_t* cycles) {
+  int best = 1;
+  *cycles = INT64_MAX;
+  for (int s = 1; s <= kMaxSplits && s <= blocks && (s == 1 || s * tiles <= 2 * sms); ++s) {
+    const bool alone = s * tiles <= sms;
+    const int64_t cost = (alone ? 7500 : 10000) + (alone ? 650 : 1000) * ((blocks + s - 1) / s);
+    if (cost < *cycles) {
+      *cycles = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 template <int kAct>
@@ -804,7 +826,8 @@ cudaError_t few_rows_launch(const Fp8Operand& a, const Fp8Operand& w, int m, int
   const int blocks = (k + kFp8Block - 1) / kFp8Block;
   const int64_t tn = (n + kTileRows - 1) / kTileRows, tm = (m + kAct - 1) / kAct;
   if (tm > 65535) return cudaErrorInvalidValue;
-  const int splits = few_splits(tn * tm, blocks, sms);
+  int64_t cycles = 0;
+  const int splits = few_splits(tn * tm, blocks, sms, &cycles);
   return launch_overlapped(few_rows_kernel<kAct>, dim3((unsigned)(tn * splits), (unsigned)tm), kFewThreads,
                            Few<kAct>::kSmem, splits, stream, tw, ta, blocks, a.scale, a.scale_row, a.scale_col,
                            w.scale, w.scale_row, w.scale_col, m, n, y, ldy, y_type, splits, error_flag);
@@ -914,15 +937,14 @@ cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, in
   int64_t cycles = 0;
   e = choose_splits(tiles, blocks, &splits, &cycles);
   if (e != cudaSuccess) return e;
-  // Tiles of 64 activation rows take 7500 cycles and 650 a block while the SMs
-  // hold one CTA each (1000 with two): shorter where the wide tiles would be few
-  // and their parts many.  128 x 4096 x 4096: 10.7 us against 14.1; 128 x 4096 x
-  // 14336: 26.8 against 19.9; 512 x 1024 x 4096: 11.4 against 13.4.
+  // Tiles of 64 activation rows are shorter where the wide ones would be few and
+  // their parts many.  128 x 4096 x 4096: 10.2 us against 13.3; 128 x 4096 x
+  // 14336: 26.8 against 19.9; 512 x 1024 x 4096: 10.1 against 12.4.
   const int64_t few = (m + 63) / 64 * ((n + kTileRows - 1) / kTileRows);
   if (2 * few <= sms) {
-    const int s = few_splits(few, blocks, sms);
-    if (7500 + (s * few <= sms ? 650 : 1000) * ((blocks + s - 1) / s) < cycles)
-      return few_rows_launch<64>(LLVQ_CALL, stream);
+    int64_t few_cycles = 0;
+    few_splits(few, blocks, sms, &few_cycles);
+    if (few_cycles < cycles) return few_rows_launch<64>(LLVQ_CALL, stream);
   }
   return wide_launch<1>(LLVQ_CALL, splits, stream);
 #undef LLVQ_CALL

@@ -296,7 +296,7 @@ def test_gemm_writes_only_its_output(m, n, k):
 
     a, sa, w, sw = operands(m, n, k)
     for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
-        for ld in (n + 3, (n + 15) // 16 * 16 + 16):
+        for ld in (n + 3, (n + 15) // 16 * 16 + 16, (n + 3) // 4 * 4 + 4, (n + 1) // 2 * 2 + 2, n | 1):
             y = torch.full((m + 2, ld), -7.0, dtype=dtype, device="cuda")
             flag = torch.zeros(1, dtype=torch.int32, device="cuda")
             _native.fp8_gemm(a.data_ptr(), a.stride(0), sa.data_ptr(), sa.stride(0), sa.stride(1), w.data_ptr(),
