@@ -116,31 +116,33 @@ __device__ __forceinline__ Raw<T> pack(const F2 (&v)[kPairs]) {
 // at a time (8 or 4: every step starts on its boundary, 16 bytes at most, and
 // the columns are a multiple of it; 1: nothing is known), by predicated loads
 // without branches, so that all the loads of a thread are in flight together.
+// Plain loads, no __restrict__ on the pointers they come from and no read-only
+// path: this kernel starts while the one ahead of it may still write what p points
+// to, so nothing is constant for the kernel's lifetime and no load may be moved
+// ahead of wait_for_inputs().
 template <typename T, int kStep>
 __device__ __forceinline__ Raw<T> load_vec(const T* p, int valid) {
   Raw<T> r;
   if constexpr (kStep * sizeof(T) >= 16) {
 #pragma unroll
     for (int i = 0; i < Raw<T>::kWords / 4; ++i) {
-      const bool in = i * 16 < valid * (int)sizeof(T);
-      const uint4 q = in ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+      const uint4 q = i * 16 < valid * (int)sizeof(T) ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
       r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
     }
   } else if constexpr (kStep * sizeof(T) == 8) {
 #pragma unroll
     for (int i = 0; i < Raw<T>::kWords / 2; ++i) {
-      const bool in = i * 8 < valid * (int)sizeof(T);
-      const uint2 q = in ? __ldg(reinterpret_cast<const uint2*>(p) + i) : make_uint2(0, 0);
+      const uint2 q = i * 8 < valid * (int)sizeof(T) ? reinterpret_cast<const uint2*>(p)[i] : make_uint2(0, 0);
       r.w[2 * i] = q.x, r.w[2 * i + 1] = q.y;
     }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) r.w[i] = i < valid ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+    for (int i = 0; i < kVec; ++i) r.w[i] = i < valid ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
   } else {
     const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
     for (int i = 0; i < kVec / 2; ++i) {
-      const uint32_t lo = 2 * i < valid ? __ldg(s + 2 * i) : 0u, hi = 2 * i + 1 < valid ? __ldg(s + 2 * i + 1) : 0u;
+      const uint32_t lo = 2 * i < valid ? s[2 * i] : 0u, hi = 2 * i + 1 < valid ? s[2 * i + 1] : 0u;
       r.w[i] = lo | hi << 16;
     }
   }
@@ -349,8 +351,8 @@ template <typename T, bool kGated>
 constexpr int kRowUnits = sizeof(T) == 4 ? 1 : 2;
 
 template <typename T, bool kGated, int kStep>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* __restrict__ x, int64_t ldx,
-                                                           const T* __restrict__ up, int64_t ldu, uint32_t rows,
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t ldx, const T* up,
+                                                           int64_t ldu, uint32_t rows,
                                                            uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
                                                            int64_t cols, Fp8Out out) {
   dependents_may_start();
@@ -406,7 +408,7 @@ constexpr int kBlockRowsPass = kBlockThreads / kGroup;       // 32 rows a pass
 constexpr int kBlockPasses = kFp8Block / kBlockRowsPass;     // 4
 
 template <typename T, int kStep>
-__global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
+__global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* x, int64_t ldx, int64_t rows,
                                                                int64_t cols, uint32_t col_blocks, Fp8Out out) {
   dependents_may_start();
   __shared__ float red[kBlockThreads / 32];
@@ -453,14 +455,17 @@ __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* __restri
 // Three shapes: up to 8192 columns one chunk, up to 16,384 two, with at most 512
 // threads and the next row in registers; beyond, two chunks of up to 1024
 // threads, which leave no registers for it.  (One chunk of 688 threads, for 11008
-// columns, left an SM with a single CTA: 63 us against the two chunks' 56 for
-// 4096 rows.)
+// columns, left an SM with a single CTA: 63 us against the two chunks' 58 for
+// 4096 rows.)  8192 x 4096 with a residual runs at 6.3 TB/s.
 template <typename T, typename W, int kChunks, int kThreads, bool kResidual, int kStep>
 __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
-    rms_norm_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ residual, int64_t ldr,
-                    const W* __restrict__ weight, float eps, float inv_cols, int64_t rows, int64_t cols,
-                    T* __restrict__ hidden, int64_t ldh, Fp8Out out) {
+    rms_norm_kernel(const T* x, int64_t ldx, const T* residual, int64_t ldr, const W* weight, float eps, float inv_cols, int64_t rows, int64_t cols,
+                    T* hidden, int64_t ldh, Fp8Out out) {
   constexpr bool kAhead = kThreads == 512 && sizeof(T) == 2;  // fp32 rows would spill
+  // The next row's loads go out ahead of the barrier, or behind it where a
+  // residual's would spill (8192 x 4096: 37.2 us against 39.3; without a residual
+  // 20.0 against 18.9).
+  constexpr bool kLate = kChunks == 1 && kResidual;
   dependents_may_start();
   __shared__ float red[2][32];
   Raw<T> rx[kChunks], rr[kChunks];
@@ -475,6 +480,11 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
   };
   wait_for_inputs();
   if constexpr (kAhead) load(blockIdx.x);
+  // the weights of a single chunk stay in registers where those reach
+  constexpr bool kHold = kChunks == 1 && !(kAhead && kResidual);
+  Raw<W> rw;
+  auto load_weight = [&](int64_t c, int valid) { rw = load_vec<W, kStep>(weight + (valid ? c : 0), valid); };
+  if constexpr (kHold) load_weight((int64_t)threadIdx.x * kVec, valid_of(cols, (int64_t)threadIdx.x * kVec));
   int side = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, side ^= 1) {
     F2 h[kChunks][kPairs], squares = pair(0.f);
@@ -492,7 +502,6 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
       for (int i = 0; i < kPairs; ++i) squares = fma(h[j][i], h[j][i], squares);
     }
     float ss = halves(squares).x + halves(squares).y;
-    if constexpr (kAhead) load(row + gridDim.x);
     if constexpr (kResidual) {
 #pragma unroll
       for (int j = 0; j < kChunks; ++j) {
@@ -504,18 +513,20 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
 #pragma unroll
     for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if ((threadIdx.x & 31) == 0) red[side][threadIdx.x >> 5] = ss;
+    if constexpr (kAhead && !kLate) load(row + gridDim.x);
     __syncthreads();  // the other side is written next: one barrier a row
     // every warp adds the warps' sums in the same tree
     float total = (threadIdx.x & 31) < blockDim.x / 32 ? red[side][threadIdx.x & 31] : 0.f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if constexpr (kAhead && kLate) load(row + gridDim.x);
     const float var = fmaf(total, inv_cols, eps);
     const float rstd = inverse_root(var);
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
       const int valid = valid_of(cols, c);
-      const Raw<W> rw = load_vec<W, kStep>(weight + (valid ? c : 0), valid);
+      if constexpr (!kHold) load_weight(c, valid);
       F2 y[kPairs];
       unpack(rw, y);
 #pragma unroll
