@@ -252,6 +252,7 @@ at::Tensor operand(PyObject* o, const char* name, int64_t* ld) {
   const at::Tensor& q = tensor(o, name);
   if (!q.is_cuda() || q.scalar_type() != at::kFloat8_e4m3fn || q.dim() != 2)
     value_error(std::string(name) + " must be a float8_e4m3fn CUDA matrix");
+  no_grad(q, name);
   const int64_t rows = q.size(0), cols = q.size(1);
   *ld = stride16(cols);
   if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && (q.stride(1) == 1 || cols <= 1)) {

@@ -341,6 +341,19 @@ def test_refusals():
         fp8.quantize_rows(x.float().requires_grad_())
 
 
+def test_eight_bit_operands_that_require_grad_are_refused():
+    from llvq_paper_reproduction_b200 import fp8
+
+    a, sa, b, sb = operands(4, 6, 256)
+    wants = a.detach().clone().requires_grad_()
+    with pytest.raises(ValueError, match="requires grad"):
+        fp8.gemm(wants, sa, b, sb)
+    with pytest.raises(ValueError, match="requires grad"):
+        fp8.gemm(a, sa, b.detach().clone().requires_grad_(), sb)
+    with torch.no_grad():
+        assert torch.equal(fp8.gemm(wants, sa, b, sb), fp8.gemm(a, sa, b, sb))
+
+
 # ------------------------------------------------------------------ as they are used
 def mlp(x, residual, norm_weight, gate_up, down):
     from llvq_paper_reproduction_b200 import fp8
@@ -449,6 +462,76 @@ def test_first_calls_inside_a_capture():
 
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and done.stdout.strip() == "fine", done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("m", [1, 40, 300, 2500])
+def test_calls_read_what_the_call_before_wrote(m):
+    """A call starts while the one ahead of it ends; the allocator hands the
+    same memory out again and again, so anything read early would be old."""
+    x0 = rand((m, 512), 5, torch.bfloat16)
+    norm_weight = rand((512,), 6, torch.bfloat16)
+    from llvq_paper_reproduction_b200 import fp8
+
+    gate_up = fp8.quantize_blocks(rand((1024, 512), 7, torch.bfloat16))
+    down = fp8.quantize_blocks(rand((512, 512), 8, torch.bfloat16))
+
+    def chain(pause):
+        x, hidden = x0, torch.zeros_like(x0)
+        for _ in range(30):
+            q, s, hidden = fp8.rms_norm(x, norm_weight, residual=hidden)
+            pause()
+            y = fp8.gemm(q, s, *gate_up)
+            pause()
+            q, s = fp8.swiglu(*y.chunk(2, dim=1))
+            pause()
+            x = fp8.gemm(q, s, *down)
+            pause()
+            q, s = fp8.quantize_rows(x)
+            pause()
+            x = x + fp8.gemm(q, s, *down)
+            pause()
+        return x, hidden
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        got = chain(lambda: None)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert bool(want[0].isfinite().all())
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_two_streams_that_join(m):
+    """Activations on one stream, the weight on another, the product behind
+    both: eagerly and as a graph with two branches, with inputs that change."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    x, w = rand((m, 768), 0, torch.bfloat16), rand((1500, 768), 1, torch.bfloat16)
+    norm_weight = torch.ones(768, device="cuda")
+    side = torch.cuda.Stream()
+
+    def forked():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        q, s = fp8.rms_norm(x, norm_weight)
+        with torch.cuda.stream(side):
+            wq, ws = fp8.quantize_blocks(w)
+        main.wait_stream(side)
+        for t in (wq, ws):
+            t.record_stream(main)
+        return fp8.gemm(q, s, wq, ws)
+
+    def plain():
+        return fp8.gemm(*fp8.rms_norm(x, norm_weight), *fp8.quantize_blocks(w), check=True)
+
+    assert torch.equal(forked(), plain())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = forked()
+    for seed in range(2, 7):
+        x.copy_(rand((m, 768), seed))
+        w.copy_(rand((1500, 768), seed + 10))
+        graph.replay()
+        assert torch.equal(y, plain())
 
 
 def test_calls_do_not_synchronise_the_host():
