@@ -395,13 +395,14 @@ struct Wide {
   static constexpr int kStageA = 128 * 128, kStageB = kTileN / kCtas * 128;
   static constexpr int kStageBytes = kStageA + kStageB;
   static constexpr int kStages = kCtas == 2 ? 5 : 4;
-  // 4 KB per adding warp to store through; a CTA with a single tile stores when its stages are free
+  // 4 KB per adding warp to store through; a CTA with a single tile stores when its stages are free, 16 KB
+  static constexpr int kStoreBufs = kCtas == 2 ? 1 : 4;
   static constexpr int kStoreOff = kCtas == 2 ? kStages * kStageBytes : 0;
   static constexpr int kScaleOff = kCtas == 2 ? kStoreOff + kAddWarps * 4096 : kStages * kStageBytes;
   static constexpr int kBarOff = kScaleOff + kScaleGroups * kScaleGroup * kScaleBlock;
   static constexpr int kBars = 2 * kStages + 2 * kAccBufs + 2 * kScaleGroups + 1;
   static constexpr size_t kSmem = (size_t)kBarOff + 8 * kBars + 16 + 1024;
-  static_assert(kSmem <= 227 * 1024 && kScaleOff >= 128 * kTileN * 4);
+  static_assert(kSmem <= 227 * 1024 && kScaleOff >= 128 * kTileN * 4 && kStoreOff + kAddWarps * kStoreBufs * 4096 <= kScaleOff);
 };
 
 // acc + v * (as ws).  Where that product comes near the ends of the range of
@@ -453,18 +454,19 @@ __device__ __forceinline__ void store_lines(const uint8_t* buf, T* __restrict__ 
   }
 }
 
-// A warp's 32 rows x kWidth columns to y, through its 4 KB of shared memory (32
-// rows of 128 bytes in the 128-byte swizzle).  Where y's rows start on 16-byte
+// A warp's 32 rows x kWidth columns to y, through kBufs times 4 KB of shared memory
+// (32 rows of 128 bytes in the 128-byte swizzle).  Where y's rows start on 16-byte
 // boundaries (tma) the buffer leaves by an asynchronous TMA store, clipped at
 // the matrix's ends; else by stores of 8, 4 or 2 bytes a lane.
-template <typename T, int kWidth>
-__device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* buf, const CUtensorMap* ty, bool tma,
+template <typename T, int kWidth, int kBufs>
+__device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* bufs, const CUtensorMap* ty, bool tma,
                                            T* __restrict__ y, int64_t ldy, int row0, int col0, int m_total, int n_total,
                                            int lane) {
   constexpr int kPerLine = 128 / (int)sizeof(T), kPerChunk = 16 / (int)sizeof(T);
 #pragma unroll
   for (int c0 = 0; c0 < kWidth; c0 += kPerLine) {
-    if (tma) {
+    uint8_t* buf = bufs + c0 / kPerLine % kBufs * 4096;
+    if (tma && kBufs * kPerLine < kWidth) {
       if (lane == 0) tc::bulk_wait_read();  // the store before has read the buffer
       __syncwarp();
     }
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAddRegs));
     const int strip = warp >> 2, quarter = warp & 3;
     const uint32_t t0 = tmem + ((uint32_t)(quarter * 32) << 16) + strip * kCols;
-    uint8_t* buf4k = base + P::kStoreOff + warp * 4096;
+    uint8_t* buf = base + P::kStoreOff + warp * (P::kStoreBufs * 4096);
     const float* scales = reinterpret_cast<const float*>(base + P::kScaleOff);
     const int my_row = quarter * 32 + lane, my_half = 128 + strip * kCols / kFp8Block;
     // Of the block's TMEM buffer, exchanged from block to block: its columns, its
@@ -718,13 +720,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           tc::st_shared4(partial_at<kTileN, true>(sbase, my_row, strip * (kCols / 4) + j), x, y_, z, w);
         }
       } else if (y_type == LLVQ_DT_F32) {
-        store_rows<float, kCols>(acc, buf4k, &ty, tma_store, static_cast<float*>(y), ldy, row0, col0, m_total, n_total,
+        store_rows<float, kCols, P::kStoreBufs>(acc, buf, &ty, tma_store, static_cast<float*>(y), ldy, row0, col0, m_total, n_total,
                                  lane);
       } else if (y_type == LLVQ_DT_F16) {
-        store_rows<__half, kCols>(acc, buf4k, &ty, tma_store, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total,
+        store_rows<__half, kCols, P::kStoreBufs>(acc, buf, &ty, tma_store, static_cast<__half*>(y), ldy, row0, col0, m_total, n_total,
                                   lane);
       } else {
-        store_rows<__nv_bfloat16, kCols>(acc, buf4k, &ty, tma_store, static_cast<__nv_bfloat16*>(y), ldy, row0, col0,
+        store_rows<__nv_bfloat16, kCols, P::kStoreBufs>(acc, buf, &ty, tma_store, static_cast<__nv_bfloat16*>(y), ldy, row0, col0,
                                          m_total, n_total, lane);
       }
     }
