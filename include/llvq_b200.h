@@ -223,11 +223,11 @@ int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_
  * its block; the last block of a row may be partial.  Scales lie anywhere:
  * scale[r * scale_row + b * scale_col] for row (or row block) r and column
  * block b.  For each block amax = max(2^-100, max |y|), scale = amax / 448,
- * byte = e4m3(448 y / amax), the quotient correctly rounded in fp32 and then
- * to e4m3 (ties to even).  NaN makes its whole block NaN; an infinity makes
+ * byte = e4m3(448 y / amax), formed in fp32 (the quantizer's quotient is
+ * correctly rounded there) and rounded to even.  NaN makes its whole block NaN; an infinity makes
  * the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
  * have a stride in elements, e4m3 rows start on 16-byte boundaries (base and
- * stride).  Device: the current one.  Nothing is allocated and no call
+ * stride).  Outputs must not overlap inputs.  Device: the current one.  Nothing is allocated and no call
  * keeps state, so calls may overlap on any streams and be captured. */
 
 /* x [rows, cols] -> q, scales of 1 x 128 blocks (block_rows = 1, activations)

@@ -359,8 +359,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
     for (int j = 0; j < kAct; j += 2) unpack2(acc[j / 2], part[j * kTileRows], part[(j + 1) * kTileRows]);
   }
-  // not earlier: CTAs of the next product placed two on one of the idle SMs would share it to their end
-  // (64 x 4096 x 14336: 20.5 us against 17.1)
+  // at the end: the next product's CTAs find no room before (at the start, 64 x 4096 x 14336: 15.0 us both)
   dependents_may_start();
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
@@ -757,8 +756,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
   }
   if (warp < kAddWarps && lane == 0) tc::bulk_wait();  // y is written before the kernel ends
-  // not earlier: CTAs of the next product placed two on one of the idle SMs would share it to their end
-  // (64 x 4096 x 14336: 20.5 us against 17.1)
+  // at the end: the next product's CTAs find no room before (at the start, 64 x 4096 x 14336: 15.0 us both)
   dependents_may_start();
   __syncwarp();
   if (failed && error_flag) atomicExch(error_flag, 1);
@@ -893,8 +891,9 @@ cudaError_t resident_clusters(int dev, int (&held)[kMaxSplits + 1]) {
 
 // CTAs per tile for Wide<1>: the shortest time over the waves of clusters, in
 // cycles as measured: 850 a block, a wave starts and stores in about 9 blocks'
-// time, and adding the parts takes 10 more (11,500 cycles for 128 rows, most of
-// them the reads of distributed shared memory).
+// time, and adding the parts takes 10 more, most of it the reads of distributed
+// shared memory.  (7 for two parts would gain 512 x 4096 x 2560, 14.1 to 13.3 us,
+// and lose 128 x 14336 x 2048, 12.6 to 13.1.)
 cudaError_t choose_splits(int64_t tiles, int64_t blocks, int* splits, int64_t* cycles) {
   int dev = 0, held[kMaxSplits + 1];
   cudaError_t e = cudaGetDevice(&dev);
@@ -965,8 +964,8 @@ cudaError_t fp8_gemm_launch(Fp8Operand a, Fp8Operand w, int64_t m, int64_t n, in
   e = choose_splits(tiles, blocks, &splits, &cycles);
   if (e != cudaSuccess) return e;
   // Tiles of 64 activation rows are shorter where the wide ones would be few and
-  // their parts many.  128 x 4096 x 4096: 10.2 us against 13.3; 128 x 4096 x
-  // 14336: 26.8 against 19.9; 512 x 1024 x 4096: 10.1 against 12.4.
+  // their parts many.  128 x 4096 x 4096: 9.9 us against 13.3; 512 x 1024 x 4096:
+  // 9.2 against 12.4; 128 x 4096 x 14336 (wide): 19.7 against 20.0.
   const int64_t few = (m + 63) / 64 * ((n + kTileRows - 1) / kTileRows);
   if (2 * few <= sms) {
     int64_t few_cycles = 0;

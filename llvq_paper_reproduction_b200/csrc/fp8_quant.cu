@@ -4,8 +4,9 @@
 //
 // For a block B of values y (1 x 128 columns, or 128 x 128 for weights):
 //   amax = max(2^-100, max |y|)      scale = amax / 448      q = e4m3(448 y / amax)
-// 448 is the largest e4m3 value, so nothing saturates; the quotient is formed
-// correctly rounded in fp32 and rounded to e4m3 once (ties to even).  NaN in
+// 448 is the largest e4m3 value, so nothing saturates; the quotient is formed in
+// fp32 (correctly rounded by the quantizers, as one product with 448 / amax by
+// norm and gate, whose y carry roundings already) and rounded to even.  NaN in
 // a block makes amax, hence the whole block, NaN; an infinity makes scale
 // infinite, its own value NaN and the others 0.  The floor 2^-100 keeps the
 // reciprocal finite: blocks below it (zeros above all) give q = 0 or values
