@@ -93,10 +93,14 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     and shape: the same bits on every call.  Scales may have any strides; 8-bit
     rows that do not start on 16-byte boundaries are copied.  Asynchronous: a
     tensor-core wait that timed out is counted in ``pending_errors``;
-    ``check=True`` synchronises and raises RuntimeError at once."""
+    ``check=True`` synchronises and raises RuntimeError at once (not while a
+    graph is captured)."""
     dtype = _TYPES.get(out_dtype)
     if dtype is None:
         raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    if check and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("check=True synchronises, which a capture cannot: capture without it, "
+                           "call raise_pending_errors after a replay")
     index = a.get_device()
     flag = _flags.get(index) or _flag(index)
     y = _ext.gemm(a, a_scale, w, w_scale, dtype, flag[1])

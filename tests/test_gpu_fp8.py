@@ -534,6 +534,21 @@ def test_two_streams_that_join(m):
         assert torch.equal(y, plain())
 
 
+def test_check_is_refused_inside_a_capture():
+    from llvq_paper_reproduction_b200 import fp8
+
+    ops = operands(5, 256, 384)
+    want = fp8.gemm(*ops, check=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            fp8.gemm(*ops, check=True)
+        y = fp8.gemm(*ops)  # the capture is still whole
+    graph.replay()
+    fp8.raise_pending_errors()
+    assert torch.equal(y, want)
+
+
 def test_calls_do_not_synchronise_the_host():
     from llvq_paper_reproduction_b200 import fp8
 
