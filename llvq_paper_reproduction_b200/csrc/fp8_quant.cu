@@ -115,8 +115,8 @@ __device__ __forceinline__ Raw<T> pack(const F2 (&v)[kPairs]) {
 
 // Sixteen elements, those from `valid` on as zeros.  kStep elements are loaded
 // at a time (8 or 4: every step starts on its boundary, 16 bytes at most, and
-// the columns are a multiple of it; 1: nothing is known), by predicated loads
-// without branches, so that all the loads of a thread are in flight together.
+// the columns are a multiple of it), by predicated loads without branches, so
+// that all the loads of a thread are in flight together.
 // Plain loads, no __restrict__ on the pointers they come from and no read-only
 // path: this kernel starts while the one ahead of it may still write what p points
 // to, so nothing is constant for the kernel's lifetime and no load may be moved
@@ -136,16 +136,6 @@ __device__ __forceinline__ Raw<T> load_vec(const T* p, int valid) {
       const uint2 q = i * 8 < valid * (int)sizeof(T) ? reinterpret_cast<const uint2*>(p)[i] : make_uint2(0, 0);
       r.w[2 * i] = q.x, r.w[2 * i + 1] = q.y;
     }
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) r.w[i] = i < valid ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-  } else {
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-    for (int i = 0; i < kVec / 2; ++i) {
-      const uint32_t lo = 2 * i < valid ? s[2 * i] : 0u, hi = 2 * i + 1 < valid ? s[2 * i + 1] : 0u;
-      r.w[i] = lo | hi << 16;
-    }
   }
   return r;
 }
@@ -161,14 +151,83 @@ __device__ __forceinline__ void store_vec(T* p, const Raw<T>& r, int valid) {
 #pragma unroll
     for (int i = 0; i < Raw<T>::kWords / 2; ++i)
       if (i * 8 < valid * (int)sizeof(T)) reinterpret_cast<uint2*>(p)[i] = make_uint2(r.w[2 * i], r.w[2 * i + 1]);
-  } else if constexpr (sizeof(T) == 4) {
+  }
+}
+
+// Where nothing is known of the boundaries (kStep 1): a warp's four blocks of 128
+// columns in loads and stores of one element a lane, neighbours side by side, turned
+// through 1 KB of the warp's shared memory into sixteen elements a thread and back.
+// (Loads of a thread's own columns touched 32 sectors each: 8000 x 4097 bf16 norm
+// with a residual 216 us against 84, rows 47 against 24, gate 79 against 44,
+// 128 x 128 blocks 38 against 26.)
+// unit(u, &left): block u's first element and its columns in the matrix, 0..128.
+constexpr int kTurnBytes = 1024;
+
+template <typename T>
+using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+
+// The loads, all in flight together ...
+template <typename T>
+struct Loaded {
+  Bits<T> v[kVec];
+  template <typename Unit>
+  __device__ __forceinline__ explicit Loaded(Unit unit) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (i < valid) reinterpret_cast<uint32_t*>(p)[i] = r.w[i];
-  } else {
+    for (int u = 0; u < 4; ++u) {
+      int left;
+      const Bits<T>* p = reinterpret_cast<const Bits<T>*>(unit(u, left));
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (i < valid) reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(r.w[i / 2] >> (16 * (i & 1)));
+      for (int j = 0; j < 4; ++j) v[u * 4 + j] = j * 32 + lane < left ? p[j * 32 + lane] : (Bits<T>)0;
+    }
+  }
+};
+
+// ... and what they brought, as the threads work on it.
+template <typename T>
+__device__ __forceinline__ Raw<T> turned(uint8_t* turn, const Loaded<T>& in) {
+  constexpr int kUnits = kTurnBytes / (kFp8Block * (int)sizeof(T));  // blocks a pass, of 4
+  const int lane = threadIdx.x & 31;
+  Raw<T> r;
+#pragma unroll
+  for (int pass = 0; pass < 4 / kUnits; ++pass) {
+    __syncwarp();  // what was there before has been read
+#pragma unroll
+    for (int i = 0; i < kUnits * 4; ++i) reinterpret_cast<Bits<T>*>(turn)[i * 32 + lane] = in.v[pass * kUnits * 4 + i];
+    __syncwarp();
+    if (lane / (kUnits * kGroup) == pass) {
+#pragma unroll
+      for (int i = 0; i < Raw<T>::kWords / 4; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(turn)[(lane % (kUnits * kGroup)) * (Raw<T>::kWords / 4) + i];
+        r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+      }
+    }
+  }
+  return r;
+}
+
+template <typename T, typename Unit>
+__device__ __forceinline__ void store_turned(uint8_t* turn, const Raw<T>& r, Unit unit) {
+  constexpr int kUnits = kTurnBytes / (kFp8Block * (int)sizeof(T));
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int pass = 0; pass < 4 / kUnits; ++pass) {
+    __syncwarp();
+    if (lane / (kUnits * kGroup) == pass) {
+#pragma unroll
+      for (int i = 0; i < Raw<T>::kWords / 4; ++i)
+        reinterpret_cast<uint4*>(turn)[(lane % (kUnits * kGroup)) * (Raw<T>::kWords / 4) + i] =
+            make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      int left;
+      Bits<T>* p = reinterpret_cast<Bits<T>*>(unit(pass * kUnits + u, left));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j * 32 + lane < left) p[j * 32 + lane] = reinterpret_cast<const Bits<T>*>(turn)[(u * 4 + j) * 32 + lane];
+    }
   }
 }
 
@@ -348,8 +407,8 @@ __device__ __forceinline__ F2 silu(F2 g) {
 // eight: what a thread spends once on a unit (three shuffles, the quotient, the
 // addresses) was half of its instructions.  kGated: y = gate / (1 + exp(-gate)) * up.
 constexpr int kRowThreads = 256;
-template <typename T, bool kGated>
-constexpr int kRowUnits = sizeof(T) == 4 ? 1 : 2;
+template <typename T, bool kGated, int kStep>
+constexpr int kRowUnits = sizeof(T) == 4 || kStep == 1 ? 1 : 2;
 
 template <typename T, bool kGated, int kStep>
 __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t ldx, const T* up,
@@ -357,7 +416,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t l
                                                            uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
                                                            int64_t cols, Fp8Out out) {
   dependents_may_start();
-  constexpr int kUnits = kRowUnits<T, kGated>;
+  constexpr int kUnits = kRowUnits<T, kGated, kStep>;
   constexpr int kTeams = kRowThreads / kGroup;
   const uint32_t first = blockIdx.x * (kTeams * kUnits) + threadIdx.x / kGroup;
   const int in_block = (int)(threadIdx.x % kGroup) * kVec;
@@ -377,8 +436,29 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t l
     }
     const int64_t c = (int64_t)b[j] * kFp8Block + in_block;
     valid[j] = row[j] < rows ? valid_of(cols, c) : 0;  // no early return: the whole warp meets in the shuffles
-    rx[j] = load_vec<T, kStep>(x + (valid[j] ? row[j] * ldx + c : 0), valid[j]);
-    if constexpr (kGated) ru[j] = load_vec<T, kStep>(up + (valid[j] ? row[j] * ldu + c : 0), valid[j]);
+    if constexpr (kStep > 1) {
+      rx[j] = load_vec<T, kStep>(x + (valid[j] ? row[j] * ldx + c : 0), valid[j]);
+      if constexpr (kGated) ru[j] = load_vec<T, kStep>(up + (valid[j] ? row[j] * ldu + c : 0), valid[j]);
+    } else {
+      __shared__ alignas(16) uint8_t turn[kRowThreads / 32][kTurnBytes];
+      const int64_t left = row[j] < rows ? cols - (int64_t)b[j] * kFp8Block : 0;
+      auto load = [&](const T* m, int64_t ld) {
+        const T* mine = m + (left > 0 ? row[j] * ld + (int64_t)b[j] * kFp8Block : 0);
+        return Loaded<T>([&](int u, int& n) {
+          n = __shfl_sync(0xffffffffu, (int)(left < kFp8Block ? left : kFp8Block), u * kGroup);
+          return reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), u * kGroup));
+        });
+      };
+      uint8_t* turning = turn[threadIdx.x / 32];
+      const Loaded<T> lx = load(x, ldx);
+      if constexpr (kGated) {
+        const Loaded<T> lu = load(up, ldu);
+        rx[j] = turned<T>(turning, lx);
+        ru[j] = turned<T>(turning, lu);
+      } else {
+        rx[j] = turned<T>(turning, lx);
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
@@ -422,8 +502,19 @@ __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* x, int64
 #pragma unroll
   for (int p = 0; p < kBlockPasses; ++p) {
     const int64_t r = r0 + p * kBlockRowsPass;
-    const int live = r < rows ? valid : 0;
-    raw[p] = load_vec<T, kStep>(x + (live ? r * ldx + c : 0), live);
+    if constexpr (kStep > 1) {
+      const int live = r < rows ? valid : 0;
+      raw[p] = load_vec<T, kStep>(x + (live ? r * ldx + c : 0), live);
+    } else {
+      __shared__ alignas(16) uint8_t turn[kBlockThreads / 32][kTurnBytes];
+      const int64_t c0 = (int64_t)cb * kFp8Block, first = r - (threadIdx.x % 32) / kGroup;  // the warp's four rows
+      const int width = (int)min(cols - c0, (int64_t)kFp8Block);
+      const Loaded<T> in([&](int u, int& n) {
+        n = first + u < rows ? width : 0;
+        return x + (n ? (first + u) * ldx + c0 : 0);
+      });
+      raw[p] = turned<T>(turn[threadIdx.x / 32], in);
+    }
   }
   float m = 0.f;
 #pragma unroll
@@ -455,28 +546,46 @@ __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* x, int64
 // The norm uses the unrounded sum h.  Threads past the row hold zeros.
 // Three shapes: up to 8192 columns one chunk, up to 16,384 two, with at most 512
 // threads and the next row in registers; beyond, two chunks of up to 1024
-// threads, which leave no registers for it.  (One chunk of 688 threads, for 11008
+// threads, which leave no registers for it.  (Rows on odd boundaries: norm_typed.)  (One chunk of 688 threads, for 11008
 // columns, left an SM with a single CTA: 63 us against the two chunks' 58 for
 // 4096 rows.)  8192 x 4096 with a residual runs at 6.3 TB/s.
+// Registers a thread: as few as leave nothing, or little, spilled.
+constexpr int norm_regs(int chunks, int threads, int step) {
+  return threads == 1024 ? 64 : chunks == 2 ? 88 : step == 1 ? 80 : 64;
+}
+
 template <typename T, typename W, int kChunks, int kThreads, bool kResidual, int kStep>
-__global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
-    rms_norm_kernel(const T* x, int64_t ldx, const T* residual, int64_t ldr, const W* weight, float eps, float inv_cols, int64_t rows, int64_t cols,
-                    T* hidden, int64_t ldh, Fp8Out out) {
-  constexpr bool kAhead = kThreads == 512 && sizeof(T) == 2;  // fp32 rows would spill
+__global__ void __maxnreg__(norm_regs(kChunks, kThreads, kStep))
+    rms_norm_kernel(const T* x, int64_t ldx, const T* residual, int64_t ldr, const W* weight, float eps,
+                    float inv_cols, int64_t rows, int64_t cols, T* hidden, int64_t ldh, Fp8Out out) {
+  constexpr bool kAhead = kThreads == 512 && sizeof(T) == 2 && kStep > 1;  // fp32 rows would spill
   // The next row's loads go out ahead of the barrier, or behind it where a
   // residual's would spill (8192 x 4096: 37.2 us against 39.3; without a residual
   // 20.0 against 18.9).
   constexpr bool kLate = kChunks == 1 && kResidual;
   dependents_may_start();
   __shared__ float red[2][32];
+  __shared__ alignas(16) uint8_t turn[kStep == 1 ? kThreads / 32 : 1][kTurnBytes];
+  // the four blocks of this warp in chunk j of a row that starts at p
+  auto blocks_of = [&](auto* p, int j) {
+    const int64_t c0 = (((int64_t)j * blockDim.x + threadIdx.x) & ~31LL) * kVec;
+    return [p, c0, cols](int u, int& n) {
+      const int64_t c = c0 + u * kFp8Block, left = cols - c;
+      n = left <= 0 ? 0 : left < kFp8Block ? (int)left : kFp8Block;
+      return p + (n ? c : 0);
+    };
+  };
+  uint8_t* mine = turn[kStep == 1 ? threadIdx.x / 32 : 0];
   Raw<T> rx[kChunks], rr[kChunks];
   auto load = [&](int64_t row) {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
       const int valid = row < rows ? valid_of(cols, c) : 0;
-      rx[j] = load_vec<T, kStep>(x + (valid ? row * ldx + c : 0), valid);
-      if constexpr (kResidual) rr[j] = load_vec<T, kStep>(residual + (valid ? row * ldr + c : 0), valid);
+      if constexpr (kStep > 1) {
+        rx[j] = load_vec<T, kStep>(x + (valid ? row * ldx + c : 0), valid);
+        if constexpr (kResidual) rr[j] = load_vec<T, kStep>(residual + (valid ? row * ldr + c : 0), valid);
+      }
     }
   };
   wait_for_inputs();
@@ -484,14 +593,24 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
   // the weights of a single chunk stay in registers where those reach
   constexpr bool kHold = kChunks == 1 && !(kAhead && kResidual);
   Raw<W> rw;
-  auto load_weight = [&](int64_t c, int valid) { rw = load_vec<W, kStep>(weight + (valid ? c : 0), valid); };
-  if constexpr (kHold) load_weight((int64_t)threadIdx.x * kVec, valid_of(cols, (int64_t)threadIdx.x * kVec));
+  auto load_weight = [&](int j) {
+    const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
+    const int valid = valid_of(cols, c);
+    if constexpr (kStep > 1) rw = load_vec<W, kStep>(weight + (valid ? c : 0), valid);
+    else rw = turned<W>(mine, Loaded<W>(blocks_of(weight, j)));
+  };
+  if constexpr (kHold) load_weight(0);
   int side = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, side ^= 1) {
     F2 h[kChunks][kPairs], squares = pair(0.f);
-    if constexpr (!kAhead) load(row);
+    if constexpr (!kAhead && kStep > 1) load(row);
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
+      if constexpr (kStep == 1) {
+        // one after the other: both in flight would spill (2047 x 16001 with a residual 107 us against 87)
+        rx[j] = turned<T>(mine, Loaded<T>(blocks_of(x + row * ldx, j)));
+        if constexpr (kResidual) rr[j] = turned<T>(mine, Loaded<T>(blocks_of(residual + row * ldr, j)));
+      }
       unpack(rx[j], h[j]);
       if constexpr (kResidual) {
         F2 r[kPairs];
@@ -508,7 +627,8 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
       for (int j = 0; j < kChunks; ++j) {
         const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
         const int valid = valid_of(cols, c);
-        store_vec<T, kStep>(hidden + (valid ? row * ldh + c : 0), pack<T>(h[j]), valid);
+        if constexpr (kStep > 1) store_vec<T, kStep>(hidden + (valid ? row * ldh + c : 0), pack<T>(h[j]), valid);
+        else store_turned<T>(mine, pack<T>(h[j]), blocks_of(hidden + row * ldh, j));
       }
     }
 #pragma unroll
@@ -527,7 +647,7 @@ __global__ void __maxnreg__(kChunks == 2 && kThreads == 512 ? 88 : 64)
     for (int j = 0; j < kChunks; ++j) {
       const int64_t c = ((int64_t)j * blockDim.x + threadIdx.x) * kVec;
       const int valid = valid_of(cols, c);
-      if constexpr (!kHold) load_weight(c, valid);
+      if constexpr (!kHold) load_weight(j);
       F2 y[kPairs];
       unpack(rw, y);
 #pragma unroll
@@ -551,7 +671,7 @@ int step_of(const void* p, int64_t ld, int64_t cols) {
 template <typename T, bool kGated, int kStep>
 cudaError_t rows_step(Fp8In x, Fp8In up, int64_t rows, int64_t cols, Fp8Out out, cudaStream_t stream) {
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block, units = rows * blocks;
-  constexpr int kTeams = kRowThreads / kGroup, kCta = kTeams * kRowUnits<T, kGated>;
+  constexpr int kTeams = kRowThreads / kGroup, kCta = kTeams * kRowUnits<T, kGated, kStep>;
   if (units > kFp8MaxUnits) return cudaErrorInvalidValue;
   return launch_overlapped(rows_kernel<T, kGated, kStep>, dim3((unsigned)((units + kCta - 1) / kCta)), kRowThreads, 0, 0,
                            stream, static_cast<const T*>(x.ptr), x.ld, static_cast<const T*>(up.ptr), up.ld,
@@ -600,33 +720,39 @@ cudaError_t norm_step(const NormCall& n) {
   int sms = 0;
   const cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
-  const int64_t resident = (int64_t)sms * std::max(1, (kChunks == 1 ? 1024 : 704) / threads);  // one wave
+  const int64_t resident = (int64_t)sms * std::max(1, 65536 / norm_regs(kChunks, kThreads, kStep) / threads);  // one wave
   return launch_overlapped(kernel, dim3((unsigned)std::min(n.rows, resident)), threads, 0, 0, n.stream,
                            static_cast<const T*>(n.x.ptr), n.x.ld, static_cast<const T*>(n.residual.ptr), n.residual.ld,
                            static_cast<const W*>(n.weight), n.eps, 1.f / (float)n.cols, n.rows, n.cols,
                            static_cast<T*>(n.hidden), n.ldh, n.out);
 }
 
-template <typename T, typename W, int kChunks, int kThreads>
+template <typename T, typename W, int kChunks, int kThreads, int kStep>
 cudaError_t norm_chunks(const NormCall& n) {
-  int step = std::min(step_of<T>(n.x.ptr, n.x.ld, n.cols), step_of<W>(n.weight, 0, n.cols));
-  if (n.residual.ptr)
-    step = std::min({step, step_of<T>(n.residual.ptr, n.residual.ld, n.cols), step_of<T>(n.hidden, n.ldh, n.cols)});
-  if (n.residual.ptr) {
-    if (step == 8) return norm_step<T, W, kChunks, kThreads, true, 8>(n);
-    if (step == 4) return norm_step<T, W, kChunks, kThreads, true, 4>(n);
-    return norm_step<T, W, kChunks, kThreads, true, 1>(n);
-  }
-  if (step == 8) return norm_step<T, W, kChunks, kThreads, false, 8>(n);
-  if (step == 4) return norm_step<T, W, kChunks, kThreads, false, 4>(n);
-  return norm_step<T, W, kChunks, kThreads, false, 1>(n);
+  return n.residual.ptr ? norm_step<T, W, kChunks, kThreads, true, kStep>(n)
+                        : norm_step<T, W, kChunks, kThreads, false, kStep>(n);
+}
+
+template <typename T, typename W, int kStep>
+cudaError_t norm_shape(const NormCall& n) {
+  if (n.cols <= 512 * kVec) return norm_chunks<T, W, 1, 512, kStep>(n);
+  if (n.cols <= 1024 * kVec) return norm_chunks<T, W, 2, 512, kStep>(n);
+  return norm_chunks<T, W, 2, 1024, kStep>(n);
 }
 
 template <typename T, typename W>
 cudaError_t norm_typed(const NormCall& n) {
-  if (n.cols <= 512 * kVec) return norm_chunks<T, W, 1, 512>(n);
-  if (n.cols <= 1024 * kVec) return norm_chunks<T, W, 2, 512>(n);
-  return norm_chunks<T, W, 2, 1024>(n);
+  int step = std::min(step_of<T>(n.x.ptr, n.x.ld, n.cols), step_of<W>(n.weight, 0, n.cols));
+  if (n.residual.ptr)
+    step = std::min({step, step_of<T>(n.residual.ptr, n.residual.ld, n.cols), step_of<T>(n.hidden, n.ldh, n.cols)});
+  if (step == 8) return norm_shape<T, W, 8>(n);
+  if (step == 4) return norm_shape<T, W, 4>(n);
+  // Turned loads are not ahead of their row: one chunk of more threads (2047 x
+  // 16001: 40 us against 51 for two of half as many), which with a residual need
+  // more registers than 1024 can have (8000 x 4097: 84 us against 99, and without
+  // a residual 43 against 36).
+  if (n.cols > 1024 * kVec) return norm_chunks<T, W, 2, 1024, 1>(n);
+  return n.residual.ptr && n.cols <= 512 * kVec ? norm_step<T, W, 1, 512, true, 1>(n) : norm_chunks<T, W, 1, 1024, 1>(n);
 }
 
 }  // namespace

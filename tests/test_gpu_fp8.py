@@ -155,6 +155,36 @@ def test_rms_norm(shape, dtype, residual, wide_weight):
         assert out[2].dtype == dtype and torch.equal(out[2], (x.float() + r.float()).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2000, 1001), (3, 2047), (131, 4097), (3, 9001), (2, 16383), (2, 16385), (2, 32767)])
+def test_rows_on_odd_boundaries(shape, dtype):
+    """Rows that start anywhere, NaN on both sides of each: nothing beside a
+    row is read into it, nothing beside the hidden row is written."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    m, k = shape
+
+    def odd(seed):
+        base = torch.full((m, k + 5 + k % 2), float("nan"), device="cuda", dtype=dtype)
+        base[:, 3:3 + k] = rand(shape, seed, dtype)
+        return base[:, 3:3 + k]
+
+    x, r, w = odd(50), odd(51), (1 + 0.1 * rand((k + 1,), 52)).to(dtype)[1:]
+    for residual in (None, r):
+        out = fp8.rms_norm(x, w, residual=residual)
+        h = x.double() + (0.0 if residual is None else r.double())
+        y = h * w.double() / torch.sqrt(h.square().mean(dim=1, keepdim=True) + 1e-5)
+        check_quantized(out[0], out[1], y, 1, NORM_REL)
+    assert torch.equal(out[2], (x.float() + r.float()).to(dtype))
+    q, scale = fp8.quantize_rows(x)
+    check_quantized(q, scale, x.double(), 1, 0.0)
+    q, scale = fp8.quantize_blocks(x)
+    check_quantized(q, scale, x.double(), BLOCK, 0.0)
+    q, scale = fp8.swiglu(x, r)
+    g = x.double()
+    check_quantized(q, scale, g * torch.sigmoid(g) * r.double(), 1, SWIGLU_REL)
+
+
 def test_rms_norm_strides_zero_rows_and_nan():
     from llvq_paper_reproduction_b200 import fp8
 
