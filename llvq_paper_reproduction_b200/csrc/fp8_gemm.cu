@@ -452,28 +452,66 @@ __device__ __forceinline__ void add_scaled(uint64_t* acc, uint32_t* v, const Sca
   for (int j = 0; j < kCount / 2; ++j) acc[j] = fma2(pack2(v[2 * j], v[2 * j + 1]), ff, acc[j]);
 }
 
-// The buffer of store_rows by stores of sizeof(U) bytes, on whose boundaries y's rows start.
-template <typename T, typename U>
-__device__ __forceinline__ void store_lines(const uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0, int col0,
-                                            int m_total, int n_total, int lane) {
-  constexpr int kPer = (int)(sizeof(U) / sizeof(T)), kLanes = 128 / (int)sizeof(U);  // lanes a row, 64 for 2 bytes
-  constexpr int kRows = kLanes < 32 ? 32 / kLanes : 1;
+// The buffer of store_rows where y's rows start on 8-byte boundaries: 16 lanes a row.
+template <typename T>
+__device__ __forceinline__ void store_halves(const uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0, int col0,
+                                             int m_total, int n_total, int lane) {
+  constexpr int kPer = 8 / (int)sizeof(T);
+  const int byte = (lane & 15) * 8, col = col0 + (lane & 15) * kPer;
+  if (col >= n_total) return;
 #pragma unroll 4
-  for (int r = kLanes < 32 ? lane / kLanes : 0; r < 32; r += kRows) {
+  for (int r = lane >> 4; r < 32; r += 2) {
+    if (row0 + r >= m_total) continue;
+    const uint2 v = *reinterpret_cast<const uint2*>(buf + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15));
+    T* dst = y + (int64_t)(row0 + r) * ldy + col;
+    if (col + kPer <= n_total) {
+      *reinterpret_cast<uint2*>(dst) = v;
+    } else {
+      const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int l = lane % kLanes; l < kLanes; l += 32) {
-      const int byte = l * (int)sizeof(U), col = col0 + l * kPer;
-      if (row0 + r >= m_total || col >= n_total) continue;
-      const U v = *reinterpret_cast<const U*>(buf + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15));
-      T* dst = y + (int64_t)(row0 + r) * ldy + col;
-      if (col + kPer <= n_total) {
-        *reinterpret_cast<U*>(dst) = v;
-      } else {
-        const T* e = reinterpret_cast<const T*>(&v);
+      for (int j = 0; j < kPer; ++j)
+        if (col + j < n_total) dst[j] = e[j];
+    }
+  }
+}
+
+// ... and where they start anywhere: eight lanes a row, whose 128 bytes they store
+// as the 16-byte chunks of memory that lie within them, each put together from five
+// words of the buffer, and the elements before the first and behind the last chunk
+// one a lane (together one chunk's, or none).  1317 x 13418 x 152, bf16: 29.1 us,
+// by stores of four bytes 32.5; of two, at 13417, 35.5.  By store_halves 13420
+// columns take 22.7 us, so 29.1; 13416, by TMA, 14.7.
+template <typename T>
+__device__ __forceinline__ void store_shifted(const uint8_t* buf, T* __restrict__ y, int64_t ldy, int row0, int col0,
+                                              int m_total, int n_total, int lane) {
+  constexpr int kLine = 128 / (int)sizeof(T), kChunk = 16 / (int)sizeof(T);
+  const int c = lane & 7, left = min(kLine, n_total - col0), rows = min(32, m_total - row0);
+  if (left <= 0) return;
+  auto at = [&](int r, int byte) { return buf + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15); };
+  T* const y0 = y + (int64_t)row0 * ldy + col0;
+  // elements of row r before a boundary
+  auto head_of = [&](int r) {
+    return (int)((16 - (reinterpret_cast<uintptr_t>(y0 + r * ldy) & 15)) & 15) / (int)sizeof(T);
+  };
+#pragma unroll 4
+  for (int r = lane >> 3; r < 32; r += 4) {
+    const int first = head_of(r) + c * kChunk, byte = first * (int)sizeof(T);
+    uint32_t w[5];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (col + j < n_total) dst[j] = e[j];
-      }
+    for (int i = 0; i < 5; ++i) w[i] = *reinterpret_cast<const uint32_t*>(at(r, ((byte & ~3) + 4 * i) & 127));
+    const uint32_t shift = (byte & 3) * 8;
+    if (r < rows && first + kChunk <= left)
+      *reinterpret_cast<uint4*>(y0 + r * ldy + first) =
+          make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+                     __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+  }
+  for (int e = c; e < (left < kLine ? 16 : 8); e += 8) {  // twice where the matrix cuts the line off
+#pragma unroll 4
+    for (int r = lane >> 3; r < 32; r += 4) {
+      const int heads = min(head_of(r), left), end = heads + (left - heads) / kChunk * kChunk;
+      const int i = e < heads ? e : end + e - heads;
+      const T v = *reinterpret_cast<const T*>(at(r, i * (int)sizeof(T) & 127));
+      if (r < rows && i < left) y0[r * ldy + i] = v;
     }
   }
 }
@@ -481,7 +519,7 @@ __device__ __forceinline__ void store_lines(const uint8_t* buf, T* __restrict__ 
 // A warp's 32 rows x kWidth columns to y, through kBufs times 4 KB of shared memory
 // (32 rows of 128 bytes in the 128-byte swizzle).  Where y's rows start on 16-byte
 // boundaries (tma) the buffer leaves by an asynchronous TMA store, clipped at
-// the matrix's ends; else by stores of 8, 4 or 2 bytes a lane.
+// the matrix's ends; else by store_halves or store_shifted.
 template <typename T, int kWidth, int kBufs>
 __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* bufs, const CUtensorMap* ty, bool tma,
                                            T* __restrict__ y, int64_t ldy, int row0, int col0, int m_total, int n_total,
@@ -512,10 +550,10 @@ __device__ __forceinline__ void store_rows(const uint64_t* acc, uint8_t* bufs, c
       if (lane == 0 && row0 < m_total && col0 + c0 < n_total) tc::tma_store_2d(ty, col0 + c0, row0, tc::smem_addr(buf));
     } else {
       __syncwarp();
-      const uintptr_t at = reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * (int64_t)sizeof(T));
-      if (at % 8 == 0) store_lines<T, uint2>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
-      else if (at % 4 == 0) store_lines<T, uint32_t>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
-      else store_lines<T, T>(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
+      if ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(ldy * (int64_t)sizeof(T))) % 8 == 0)
+        store_halves(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
+      else
+        store_shifted(buf, y, ldy, row0, col0 + c0, m_total, n_total, lane);
       __syncwarp();
     }
   }
