@@ -565,7 +565,7 @@ __global__ void __maxnreg__(norm_regs(kChunks, kThreads, kStep))
   constexpr bool kLate = kChunks == 1 && kResidual;
   dependents_may_start();
   __shared__ float red[2][32];
-  __shared__ alignas(16) uint8_t turn[kStep == 1 ? kThreads / 32 : 1][kTurnBytes];
+  extern __shared__ __align__(16) uint8_t turn[];  // kTurnBytes a warp (kStep 1)
   // the four blocks of this warp in chunk j of a row that starts at p
   auto blocks_of = [&](auto* p, int j) {
     const int64_t c0 = (((int64_t)j * blockDim.x + threadIdx.x) & ~31LL) * kVec;
@@ -575,7 +575,7 @@ __global__ void __maxnreg__(norm_regs(kChunks, kThreads, kStep))
       return p + (n ? c : 0);
     };
   };
-  uint8_t* mine = turn[kStep == 1 ? threadIdx.x / 32 : 0];
+  uint8_t* mine = turn + threadIdx.x / 32 * kTurnBytes;
   Raw<T> rx[kChunks], rr[kChunks];
   auto load = [&](int64_t row) {
 #pragma unroll
@@ -721,7 +721,8 @@ cudaError_t norm_step(const NormCall& n) {
   const cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
   const int64_t resident = (int64_t)sms * std::max(1, 65536 / norm_regs(kChunks, kThreads, kStep) / threads);  // one wave
-  return launch_overlapped(kernel, dim3((unsigned)std::min(n.rows, resident)), threads, 0, 0, n.stream,
+  const size_t smem = kStep == 1 ? (size_t)threads / 32 * kTurnBytes : 0;
+  return launch_overlapped(kernel, dim3((unsigned)std::min(n.rows, resident)), threads, smem, 0, n.stream,
                            static_cast<const T*>(n.x.ptr), n.x.ld, static_cast<const T*>(n.residual.ptr), n.residual.ld,
                            static_cast<const W*>(n.weight), n.eps, 1.f / (float)n.cols, n.rows, n.cols,
                            static_cast<T*>(n.hidden), n.ldh, n.out);
