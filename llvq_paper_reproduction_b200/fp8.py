@@ -4,6 +4,8 @@ An 8-bit matrix is a pair (q, scale): q float8_e4m3fn [rows, cols], scale
 fp32 per block of 128 columns, value = q * scale of its block.  Activations
 have a scale per row ([rows, ceil(cols / 128)]), weights one per 128 x 128
 block ([ceil(rows / 128), ceil(cols / 128)]); last blocks may be partial.
+The operators' q have rows on 16-byte boundaries, from 1024 columns on whole
+128-byte lines, so q is a view with gaps unless its columns are such a multiple.
 
     x, hidden     -> rms_norm       -> 8-bit x      (residual addition, norm)
     8-bit x, W    -> gemm           -> gate and up
