@@ -322,11 +322,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     for (int i0 = 0; i0 < count; i0 += F::kGroup) {
       if (i0 % F::kChunk == 0) {
         tc::cp_async_wait<0>();
+        __syncwarp();
         asm volatile("bar.sync 1, 128;" ::: "memory");  // this chunk is whole, and nobody reads the last one any more
         if (i0 + F::kChunk < count) fetch(i0 / F::kChunk + 1);
       }
       const int g = i0 / F::kGroup, buf = g % F::kBufs;
       if (!seen && !failed && !tc::mbar_wait_for<0>(acc_full(buf), (g / F::kBufs) & 1)) failed = true;
+      __syncwarp();  // lanes leave a wait one by one, and a TMEM load is the whole warp's
       tc::fence_after_sync();
       uint32_t v[64];
       tc::tmem_ld64(t0 + buf * 64, v);
@@ -752,12 +754,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll 1
         for (int u = 0; u < last; ++u, ++g, slot += kScaleBlock / 4) {
           if (!seen && !failed && !tc::mbar_wait_for<0>(ready, (g >> 1) & 1u)) failed = true;
+          __syncwarp();  // lanes leave a wait one by one, and a TMEM load is the whole warp's
           tc::fence_after_sync();
           uint32_t v[64];
           tc::tmem_ld64(columns, v);
           const Scale scale(slot[my_row], slot[my_half]);
           tc::tmem_wait_ld();
           add_scaled<64>(acc, v, scale);
+          __syncwarp();  // after the branch by the lane
           tc::tmem_ld64(columns + 64, v);
           tc::tmem_wait_ld();
           tc::fence_before_sync();

@@ -1,0 +1,53 @@
+"""The 8-bit operators on the shapes whose kernels, loops and branches smaller
+calls do not reach.  Each test names the kernel it is about and asserts that
+its calls take it, so that a changed rule of choice cannot empty the test.
+Tolerances: as derived in fp8_reference.py and test_gpu_fp8.py."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cuda_launches import launches
+from fp8_reference import check_product
+
+pytestmark = pytest.mark.gpu
+
+WIDE, PAIRS = "wide_kernelILi1E", "wide_kernelILi2E"
+
+
+def rand(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def operands(m, n, k, seed=0):
+    from llvq_paper_reproduction_b200 import fp8
+
+    return *fp8.quantize_rows(rand((m, k), seed)), *fp8.quantize_blocks(rand((n, k), seed + 1, scale=0.02))
+
+
+def product(a, sa, w, sw, dtype, kernel, parts=1):
+    """fp8.gemm, which has to take `kernel` with every tile's K in `parts`."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    y = fp8.gemm(a, sa, w, sw, out_dtype=dtype, check=True)
+    (launch,) = launches(lambda: fp8.gemm(a, sa, w, sw, out_dtype=dtype))
+    assert kernel in launch.name and launch.cluster == (2 if kernel == PAIRS else parts), launch
+    return y
+
+
+# ------------------------------------------------------------------ scales and rows apart
+@pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (2500, 4200, 400, PAIRS)])
+def test_wide_rows_whose_scales_leave_the_range_beside_others(m, n, k, kernel):
+    """Every other row's scale times the weight's is below the normal fp32
+    numbers while the row's products are not: the two are applied one after the
+    other, by the lane, with the warp's other lanes on the single product."""
+    a, sa, w, sw = operands(m, n, k)
+    sw = sw * 2.0 ** -30
+    sa = sa.clone()
+    sa[1::2] *= 2.0 ** -90
+    factors = sa.double()[:, None, :] * sw.double()[None]
+    assert (factors[1::2] < 2.0 ** -126).all() and (factors[::2] > 2.0 ** -60).all()
+    y = product(a, sa, w, sw, torch.float32, kernel)
+    assert (y[1::2].abs().amax(dim=1) > 2.0 ** -126).all()
+    check_product(y, a, sa, w, sw)
