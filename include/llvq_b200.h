@@ -234,7 +234,8 @@ int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_
  * or 128 x 128 blocks (block_rows = 128, weights). */
 int llvq_fp8_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int64_t cols, int32_t block_rows,
                       uint8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_col, void* stream);
-/* y = gate / (1 + exp(-gate)) * up in fp32, quantized in 1 x 128 blocks. */
+/* y = gate / (1 + exp(-gate)) * up in fp32, quantized in 1 x 128 blocks; also
+ * for gates whose exponential fp32 cannot hold, down to -174 (0 below). */
 int llvq_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int32_t type, int64_t rows,
                     int64_t cols, uint8_t* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_col,
                     void* stream);

@@ -78,18 +78,24 @@ struct Raw {
   uint32_t w[kWords];
 };
 
+// The two 16-bit values of a word.
+template <typename T>
+__device__ __forceinline__ F2 pair_in(uint32_t word) {
+  static_assert(sizeof(T) == 2);
+  if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word));
+    return pair(f.x, f.y);
+  } else {
+    return pair(__uint_as_float(word << 16), __uint_as_float(word & 0xFFFF0000u));
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack(const Raw<T>& r, F2 (&v)[kPairs]) {
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      v[i] = pair(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
-    } else if constexpr (std::is_same_v<T, __half>) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
-      v[i] = pair(f.x, f.y);
-    } else {
-      v[i] = pair(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xFFFF0000u));
-    }
+    if constexpr (sizeof(T) == 4) v[i] = pair(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else v[i] = pair_in<T>(r.w[i]);
   }
 }
 
@@ -372,32 +378,106 @@ __device__ __forceinline__ int valid_of(int64_t cols, int64_t c) {
   return left >= kVec ? kVec : left > 0 ? (int)left : 0;
 }
 
-// gate / (1 + exp(-gate)) of a pair.  exp(-g) = 2^-n (1 + l ln 2), n = RN(g
-// kLog2e) and l what that product and the rounded constant lost (kLog2e = log2 e -
-// 1.926e-8, kTail = -1.926e-8 ln 2), so that its error is that of ex2.approx
-// (2^-22) for every g; the reciprocal takes one Newton step.  The exponent's
-// argument is kept within +-88.5 so that all of this stays finite: below g = -87.3
-// the reciprocal is flushed to zero and the quotient g * 0 (NaN for an infinite
-// g), above 88.5 it is g.
-__device__ __forceinline__ F2 silu(F2 g) {
+// exp(-c) of a pair, c within +-88.5: 2^-n (1 + l ln 2), n = RN(c kLog2e) and l
+// what that product and the rounded constant lost (kLog2e = log2 e - 1.926e-8,
+// kTail = -1.926e-8 ln 2), so that its error is that of ex2.approx (2^-22) for
+// every c; below 2^-126 it is 0.
+__device__ __forceinline__ F2 exp_minus(F2 c) {
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kTail = -1.33497582e-8f;
-  const float2 f = halves(g);
-  const F2 c = pair(fminf(fmaxf(f.x, -88.5f), 88.5f), fminf(fmaxf(f.y, -88.5f), 88.5f));
   const F2 n = c * pair(kLog2e);
   const F2 l = fma(c, pair(-kLog2e), n);
   const float2 m = halves(n);
-  float2 e, r;
+  float2 e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(-m.x));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(-m.y));
-  F2 ee = pair(e.x, e.y);
-  ee = fma(ee, fma(c, pair(kTail), l * pair(kLn2)), ee);
-  const F2 minus_d = fma(ee, pair(-1.f), pair(-1.f));
+  const F2 ee = pair(e.x, e.y);
+  return fma(ee, fma(c, pair(kTail), l * pair(kLn2)), ee);
+}
+
+__device__ __forceinline__ F2 clamped(F2 v) {
+  const float2 f = halves(v);
+  return pair(fminf(fmaxf(f.x, -88.5f), 88.5f), fminf(fmaxf(f.y, -88.5f), 88.5f));
+}
+
+// gate / (1 + exp(-gate)) of a pair; the reciprocal takes one Newton step.  The
+// exponent's argument is clamped so that all of this stays finite: below g =
+// -87.3 the reciprocal is flushed to zero and the quotient g * 0 (NaN for an
+// infinite g; low_gate() is for the finite ones), above 88.5 it is g.
+__device__ __forceinline__ F2 silu(F2 g) {
+  const F2 minus_d = fma(exp_minus(clamped(g)), pair(-1.f), pair(-1.f));
   const float2 d = halves(minus_d);
+  float2 r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(-d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(-d.y));
   F2 rr = pair(r.x, r.y);
   rr = fma(rr, fma(minus_d, rr, pair(1.f)), rr);
   return g * rr;
+}
+
+// silu(gate) up for gates below kLowGate: exp(-gate) or its reciprocal leaves
+// fp32's normal range there, and the product need not.  1 + exp(-gate) is
+// exp(-gate) to the last bit, so with E = exp(gate / 2) it is (gate E) (E up).  E
+// is 0 below gate = -174.7, where the product is below 2^-116 whatever up is.  A
+// group of sixteen asks for its smallest gate first: 64 x 14336 bf16 3.3 us, 3.1
+// without.
+constexpr float kLowGate = -87.f;
+__device__ __forceinline__ F2 low_gate(F2 gate, F2 up) {
+  const F2 e = exp_minus(clamped(gate * pair(-0.5f)));
+  return gate * e * (e * up);
+}
+
+// Smallest of the values as they lie in memory; NaN does not count.
+template <typename T>
+__device__ __forceinline__ float lowest_of(const Raw<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    float m = __uint_as_float(r.w[0]);
+#pragma unroll
+    for (int i = 1; i < Raw<T>::kWords; ++i) m = fminf(m, __uint_as_float(r.w[i]));
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 m = *reinterpret_cast<const T2*>(&r.w[0]);
+#pragma unroll
+    for (int i = 1; i < Raw<T>::kWords; ++i) m = __hmin2(m, *reinterpret_cast<const T2*>(&r.w[i]));
+    const float2 f = both(m);
+    return fminf(f.x, f.y);
+  }
+}
+
+__device__ __forceinline__ F2 any_gate(F2 gate, F2 up) {
+  const float2 g = halves(gate), low = halves(low_gate(gate, up)), y = halves(silu(gate) * up);
+  return pair(g.x < kLowGate ? low.x : y.x, g.y < kLowGate ? low.y : y.y);
+}
+
+// any_gate of sixteen: a rolled loop that works on the first pair and moves the
+// others up, results behind them, so that it takes no registers beside the inputs'.
+template <typename T>
+__device__ __forceinline__ void any_gates(F2 (&y)[kPairs], const Raw<T>& gate, const Raw<T>& up) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t a[kPairs], b[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) a[i] = gate.w[i], b[i] = up.w[i];
+#pragma unroll 1
+    for (int turn = 0; turn < kPairs; ++turn) {
+      const float2 v = halves(any_gate(pair_in<T>(a[0]), pair_in<T>(b[0])));
+#pragma unroll
+      for (int i = 0; i + 1 < kPairs; ++i) a[i] = a[i + 1], b[i] = b[i + 1];
+      a[kPairs - 1] = __float_as_uint(v.x), b[kPairs - 1] = __float_as_uint(v.y);
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) y[i] = pair(__uint_as_float(a[i]), __uint_as_float(b[i]));
+  } else {
+    F2 w[kPairs];
+    unpack(gate, y);
+    unpack(up, w);
+#pragma unroll 1
+    for (int turn = 0; turn < kPairs; ++turn) {
+      const F2 v = any_gate(y[0], w[0]);
+#pragma unroll
+      for (int i = 0; i + 1 < kPairs; ++i) y[i] = y[i + 1], w[i] = w[i + 1];
+      y[kPairs - 1] = v;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- rows
@@ -410,8 +490,13 @@ constexpr int kRowThreads = 256;
 template <typename T, bool kGated, int kStep>
 constexpr int kRowUnits = sizeof(T) == 4 || kStep == 1 ? 1 : 2;
 
+// CTAs an SM holds at least (0: not asked for).  4096 x 11008 gate, bf16: 37.6 us
+// for four, 38.4 not asked for, 40.1 for five, which spill; fp32 59.1 for five, 75.9 for six.
 template <typename T, bool kGated, int kStep>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t ldx, const T* up,
+constexpr int kRowCtas = !kGated || kStep == 1 ? 0 : sizeof(T) == 4 ? 5 : 4;
+
+template <typename T, bool kGated, int kStep>
+__global__ void __launch_bounds__(kRowThreads, kRowCtas<T, kGated, kStep>) rows_kernel(const T* x, int64_t ldx, const T* up,
                                                            int64_t ldu, uint32_t rows,
                                                            uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
                                                            int64_t cols, Fp8Out out) {
@@ -464,14 +549,19 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const T* x, int64_t l
   for (int j = 0; j < kUnits; ++j) {
     F2 v[kPairs];
     float largest;
-    unpack(rx[j], v);
     if constexpr (kGated) {
-      F2 w[kPairs];
-      unpack(ru[j], w);
+      if (lowest_of(rx[j]) < kLowGate) {  // hardly ever
+        any_gates(v, rx[j], ru[j]);
+      } else {
+        F2 w[kPairs];
+        unpack(rx[j], v);
+        unpack(ru[j], w);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) v[i] = silu(v[i]) * w[i];
+        for (int i = 0; i < kPairs; ++i) v[i] = silu(v[i]) * w[i];
+      }
       largest = amax_of(v);
     } else {
+      unpack(rx[j], v);
       largest = amax_of(rx[j]);
     }
     const std::conditional_t<kGated, Quotient, ExactQuotient> quo(group_max(largest));

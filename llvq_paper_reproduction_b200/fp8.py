@@ -70,7 +70,8 @@ def quantize_blocks(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """gate / (1 + exp(-gate)) * up in fp32, quantized as ``quantize_rows``.
+    """gate / (1 + exp(-gate)) * up in fp32, quantized as ``quantize_rows``;
+    also for gates whose exponential fp32 cannot hold, down to -174 (0 below).
     gate and up [rows, cols] may be the halves of one product's rows
     (``y.chunk(2, dim=1)``): nothing is copied."""
     return _ext.swiglu(gate, up)

@@ -51,3 +51,43 @@ def test_wide_rows_whose_scales_leave_the_range_beside_others(m, n, k, kernel):
     y = product(a, sa, w, sw, torch.float32, kernel)
     assert (y[1::2].abs().amax(dim=1) > 2.0 ** -126).all()
     check_product(y, a, sa, w, sw)
+
+
+# ------------------------------------------------------------------ the gate's lower end
+# gate / (1 + exp(-gate)) * up below gate = -87 is (gate E) (E up), E = exp(gate / 2): each E
+# within 2 units (2^-22), three products of 2^-24
+LOW_REL = 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cols", [512, 515])
+def test_swiglu_of_gates_whose_exponential_leaves_the_range(cols, dtype):
+    """From -87.3 on the reciprocal of 1 + exp(-gate) is below the normal fp32
+    numbers, from -88.8 on the exponential above the largest; with a large up the
+    product is neither (with fp16's largest, 1/14 of the floor 2^-100: a byte of 32)."""
+    from fp8_reference import check_quantized
+    from llvq_paper_reproduction_b200 import fp8
+
+    from llvq_paper_reproduction_b200.fp8 import E4M3
+
+    gate = torch.linspace(-87.0, -100.0, 6 * cols, device="cuda").view(6, cols).to(dtype)
+    gate[:, ::7] = rand((6, cols), 65, dtype)[:, ::7]  # ordinary ones among them
+    up = (rand((6, cols), 66).sign() * torch.finfo(dtype).max * 0.9).to(dtype)
+    up[:, ::7] = 1e-30 if dtype != torch.float16 else 0.0
+    g = gate.double()
+    y = g * torch.sigmoid(g) * up.double()
+    q, scale = fp8.swiglu(gate, up)
+    assert q.dtype == E4M3 and (q.float() != 0).float().mean() > (0.8 if dtype != torch.float16 else 0.05)
+    check_quantized(q, scale, y, 1, LOW_REL)
+
+
+def test_swiglu_far_below_and_not_finite():
+    from llvq_paper_reproduction_b200 import fp8
+
+    up = torch.full((1, 128), 3e38, device="cuda")
+    for low in (-200.0, -1000.0, -3e38):
+        gate = torch.full((1, 128), low, device="cuda")
+        q, scale = fp8.swiglu(gate, up)
+        assert not q.float().any() and scale.isfinite().all()
+    gate[0, 5] = float("nan")
+    assert fp8.swiglu(gate, up)[0].float().isnan().all()
