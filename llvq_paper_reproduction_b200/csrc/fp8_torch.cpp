@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -67,6 +68,8 @@ int code_of(at::ScalarType t) {
 void no_grad(const at::Tensor& x, const char* name) {
   if (x.requires_grad() && at::GradMode::is_enabled())
     value_error(std::string(name) + " requires grad: the 8-bit operators are forward only (use torch.no_grad)");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(/*level=*/0).defined())
+    value_error(std::string(name) + " carries a tangent: the 8-bit operators have no derivatives (use unpack_dual)");
 }
 
 // A 2-D CUDA matrix of a supported type whose rows are dense.

@@ -16,7 +16,7 @@ The operators' q have rows on 16-byte boundaries, from 1024 columns on whole
 Every call is one kernel on torch's current stream of the inputs' device,
 never synchronises, keeps nothing between calls and may be captured in a CUDA
 graph.  Forward only: an input that requires grad is refused while grad mode
-is on.  Checks, outputs and the call of the library are one step of compiled
+is on, one that carries a forward-mode tangent while that mode is.  Checks, outputs and the call of the library are one step of compiled
 code (``csrc/fp8_torch.cpp``), which a call on a few tokens would otherwise
 spend most of its time on.  The reference has no 8-bit path; there is no
 fallback to anything but the in-tree library.

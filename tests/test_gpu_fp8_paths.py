@@ -91,3 +91,30 @@ def test_swiglu_far_below_and_not_finite():
         assert not q.float().any() and scale.isfinite().all()
     gate[0, 5] = float("nan")
     assert fp8.swiglu(gate, up)[0].float().isnan().all()
+
+
+# ------------------------------------------------------------------ what a call may be given
+def calls(m=4, k=256, n=6):
+    """Every input of every operator: a name, the tensor, and the call with it."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    x, r, w = rand((m, k), 60), rand((m, k), 61), 1 + 0.1 * rand((k,), 62)
+    a, sa, b, sb = operands(m, n, k)
+    return [("quantize_rows x", x, fp8.quantize_rows), ("quantize_blocks w", x, fp8.quantize_blocks),
+            ("swiglu gate", x, lambda t: fp8.swiglu(t, r)), ("swiglu up", r, lambda t: fp8.swiglu(x, t)),
+            ("rms_norm x", x, lambda t: fp8.rms_norm(t, w)), ("rms_norm weight", w, lambda t: fp8.rms_norm(x, t)),
+            ("rms_norm residual", r, lambda t: fp8.rms_norm(x, w, residual=t)),
+            ("gemm a_scale", sa, lambda t: fp8.gemm(a, t, b, sb)), ("gemm w_scale", sb, lambda t: fp8.gemm(a, sa, b, t))]
+
+
+def test_inputs_with_a_tangent_are_refused():
+    """Forward only: a dual tensor's tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    for name, x, call in calls():
+        with fwd.dual_level():
+            dual = fwd.make_dual(x, torch.ones_like(x))
+            with pytest.raises(ValueError, match="tangent"):
+                call(dual)
+                pytest.fail(name)
+            call(fwd.unpack_dual(dual).primal)  # the values alone
