@@ -72,7 +72,7 @@ void no_grad(const at::Tensor& x, const char* name) {
     value_error(std::string(name) + " carries a tangent: the 8-bit operators have no derivatives (use unpack_dual)");
 }
 
-// A 2-D CUDA matrix of a supported type whose rows are dense.
+// A 2-D CUDA matrix of a supported type whose rows are dense and whose memory holds its values.
 at::Tensor input(PyObject* o, const char* name) {
   const at::Tensor& x = tensor(o, name);
   if (!x.is_cuda()) value_error(std::string(name) + " must be a CUDA tensor");
@@ -80,9 +80,10 @@ at::Tensor input(PyObject* o, const char* name) {
     value_error(std::string(name) + " must be bfloat16, float16 or float32, got " + c10::toString(x.scalar_type()));
   if (x.dim() != 2) value_error(std::string(name) + " must have two dimensions, got " + std::to_string(x.dim()));
   no_grad(x, name);
-  if (x.stride(1) == 1 || x.size(1) <= 1) return x;
+  const bool dense = x.stride(1) == 1 || x.size(1) <= 1;
+  if (dense && !x.is_neg()) return x;
   const c10::cuda::CUDAGuard guard(x.device());
-  return x.contiguous();
+  return dense ? x.resolve_neg() : x.contiguous();
 }
 
 std::string describe(const at::Tensor& x) {
@@ -241,6 +242,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const c10::cuda::CUDAGuard guard(device);
     if (!weight.is_contiguous()) weight = weight.contiguous();
+    if (weight.is_neg()) weight = weight.resolve_neg();
     const at::Tensor q = empty_e4m3(m, k, device), scale = empty_row_scales(m, k, device);
     if (with) hidden = empty({m, k}, {k, 1}, x.scalar_type(), device);
     check(g.rms_norm(x.data_ptr(), x.stride(0), with ? residual.data_ptr() : nullptr, with ? residual.stride(0) : 0,
@@ -258,6 +260,7 @@ at::Tensor operand(PyObject* o, const char* name, int64_t* ld) {
   const at::Tensor& q = tensor(o, name);
   if (!q.is_cuda() || q.scalar_type() != at::kFloat8_e4m3fn || q.dim() != 2)
     value_error(std::string(name) + " must be a float8_e4m3fn CUDA matrix");
+  if (q.is_neg()) value_error(std::string(name) + " is a view with the negative bit, which e4m3 memory has no form for");
   no_grad(q, name);
   const int64_t rows = q.size(0), cols = q.size(1);
   *ld = row_bytes(cols);
@@ -274,13 +277,15 @@ at::Tensor operand(PyObject* o, const char* name, int64_t* ld) {
   return copy;
 }
 
-const at::Tensor& scales(PyObject* o, const char* name, int64_t rows, int64_t cols, at::Device device) {
+at::Tensor scales(PyObject* o, const char* name, int64_t rows, int64_t cols, at::Device device) {
   const at::Tensor& s = tensor(o, name);
   if (s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != rows || s.size(1) != cols || s.device() != device)
     value_error(std::string(name) + " must be [" + std::to_string(rows) + ", " + std::to_string(cols) +
                 "] Float on " + device.str() + ", got " + describe(s));
   no_grad(s, name);
-  return s;
+  if (!s.is_neg()) return s;
+  const c10::cuda::CUDAGuard guard(device);
+  return s.resolve_neg();
 }
 
 // gemm(a, a_scale, w, w_scale, type code of the output, address of the error flag)
@@ -296,8 +301,8 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Device device = a.device();
     if (w.size(1) != k) value_error("a has " + std::to_string(k) + " columns, w has " + std::to_string(w.size(1)));
     if (w.device() != device) value_error("a is on " + device.str() + ", w on " + w.device().str());
-    const at::Tensor& sa = scales(args[1], "a_scale", m, blocks(k), device);
-    const at::Tensor& sw = scales(args[3], "w_scale", blocks(rows), blocks(k), device);
+    const at::Tensor sa = scales(args[1], "a_scale", m, blocks(k), device);
+    const at::Tensor sw = scales(args[3], "w_scale", blocks(rows), blocks(k), device);
     const c10::cuda::CUDAGuard guard(device);
     const at::ScalarType out = type == LLVQ_DT_F32 ? at::kFloat : type == LLVQ_DT_F16 ? at::kHalf : at::kBFloat16;
     const at::Tensor y = empty({m, rows}, {rows, 1}, out, device);

@@ -118,3 +118,21 @@ def test_inputs_with_a_tangent_are_refused():
                 call(dual)
                 pytest.fail(name)
             call(fwd.unpack_dual(dual).primal)  # the values alone
+
+
+def test_lazy_negation_is_not_lost():
+    """A view with the negative bit reads as its values; e4m3, whose bytes have no such form, is refused."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    def same(got, want):
+        for g, w in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(g.float(), w.float()), name
+
+    for name, x, call in calls():
+        same(call(torch._neg_view(x)), call(-x))
+    z = torch.complex(rand((5, 1), 63), rand((5, 1), 64))
+    same(fp8.quantize_rows(z.conj().imag), fp8.quantize_rows(-z.imag.contiguous()))
+    a, sa, b, sb = operands(4, 6, 256)
+    for bad in (lambda: fp8.gemm(torch._neg_view(a), sa, b, sb), lambda: fp8.gemm(a, sa, torch._neg_view(b), sb)):
+        with pytest.raises(ValueError):
+            bad()
