@@ -13,13 +13,16 @@ The operators' q have rows on 16-byte boundaries, from 1024 columns on whole
     any x         -> quantize_rows  -> 8-bit x
     weight        -> quantize_blocks (or LeechLatticeVectorQuantizerGpu.dequantize_fp8) -> 8-bit W
 
-Every call is one kernel on torch's current stream of the inputs' device,
-never synchronises, keeps nothing between calls and may be captured in a CUDA
-graph.  Forward only: an input that requires grad is refused while grad mode
-is on, one that carries a forward-mode tangent while that mode is.  Checks, outputs and the call of the library are one step of compiled
-code (``csrc/fp8_torch.cpp``), which a call on a few tokens would otherwise
-spend most of its time on.  The reference has no 8-bit path; there is no
-fallback to anything but the in-tree library.
+Every call is one kernel on torch's current stream of the inputs' device (one
+more for each operand that has to be copied first), never synchronises, keeps
+nothing between calls and may be captured in a CUDA graph; but the first
+product on a device makes its error flag, which is kept: that call synchronises
+once and is refused while a graph is captured.  Forward only: an input that
+requires grad is refused while grad mode is on, one that carries a forward-mode
+tangent while that mode is.  Checks, outputs and the call of the library are
+one step of compiled code (``csrc/fp8_torch.cpp``), which a call on a few
+tokens would otherwise spend most of its time on.  The reference has no 8-bit
+path; there is no fallback to anything but the in-tree library.
 """
 from __future__ import annotations
 
@@ -122,7 +125,8 @@ def _flag(index: int) -> tuple[torch.Tensor | None, int]:
     if torch.cuda.is_current_stream_capturing():
         # memory taken during a capture belongs to that graph
         raise RuntimeError("call fp8.gemm once on this device before capturing it in a CUDA graph")
-    f = torch.zeros((1,), dtype=torch.int32, device=torch.device("cuda", index))
+    with torch.inference_mode(False):  # made by a first call inside, it is cleared outside
+        f = torch.zeros((1,), dtype=torch.int32, device=torch.device("cuda", index))
     torch.cuda.synchronize(index)  # once: whichever stream sets it first
     return _flags.setdefault(index, (f, f.data_ptr()))
 

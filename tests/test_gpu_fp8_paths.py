@@ -136,3 +136,20 @@ def test_lazy_negation_is_not_lost():
     for bad in (lambda: fp8.gemm(torch._neg_view(a), sa, b, sb), lambda: fp8.gemm(a, sa, torch._neg_view(b), sb)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_first_product_in_inference_mode(monkeypatch):
+    """The error flag made there can be read and cleared outside."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    monkeypatch.setattr(fp8, "_flags", {})  # as in a fresh process
+    ops = operands(4, 6, 256)
+    with torch.inference_mode():
+        fp8.gemm(*ops)
+        ((flag, _),) = fp8._flags.values()
+        flag.fill_(1)  # as after a timeout
+    with pytest.raises(RuntimeError, match="timed out"):
+        fp8.raise_pending_errors()
+    assert fp8.pending_errors() == {"gemm_timeout": 0}
+    fp8.raise_pending_errors()
+    fp8.gemm(*ops, check=True)
