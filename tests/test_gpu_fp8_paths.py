@@ -93,6 +93,25 @@ def test_swiglu_far_below_and_not_finite():
     assert fp8.swiglu(gate, up)[0].float().isnan().all()
 
 
+@pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (2500, 4200, 400, PAIRS)])
+def test_wide_rows_of_zeros_and_of_small_numbers(m, n, k, kernel):
+    """Padding rows, whose scale is the floor's, and rows whose scale times the
+    weight's lies anywhere down to the smallest normal fp32 number or up to 2^100."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    x = rand((m, k), 2)
+    x[m // 4::3] = 0.0
+    a, sa = fp8.quantize_rows(x)
+    w, sw = fp8.quantize_blocks(rand((n, k), 3, scale=0.02))
+    sa = sa.clone()
+    exponents = torch.arange(m, device="cuda") % 230 - 118
+    live = x.any(dim=1)
+    sa[live] *= torch.exp2(exponents[live].float())[:, None] / sa[live].amax(dim=1, keepdim=True)
+    y = product(a, sa, w, sw * (2.0 ** -6 / sw.amax()), torch.float32, kernel)
+    assert not y[~live].any() and y[live].isfinite().all()
+    check_product(y, a, sa, w, sw * (2.0 ** -6 / sw.amax()))
+
+
 # ------------------------------------------------------------------ what a call may be given
 def calls(m=4, k=256, n=6):
     """Every input of every operator: a name, the tensor, and the call with it."""
