@@ -36,6 +36,30 @@ def product(a, sa, w, sw, dtype, kernel, parts=1):
     return y
 
 
+# ------------------------------------------------------------------ the product's edges
+@pytest.mark.parametrize("m,n,k,kernel", [(600, 4100, 300, WIDE), (500, 4099, 2000, WIDE), (2500, 4100, 300, PAIRS)])
+def test_wide_products_write_only_their_output(m, n, k, kernel):
+    """Through the C ABI: an output inside a wider buffer, with what lies around it left as it was."""
+    from llvq_paper_reproduction_b200 import _native
+
+    a, sa, w, sw = operands(m, n, k)
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for dtype, code in ((torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)):
+        for ld in (n + 3, (n + 15) // 16 * 16 + 16, (n + 3) // 4 * 4 + 4, (n + 1) // 2 * 2 + 2, n | 1):
+            y = torch.full((m + 2, ld), -7.0, dtype=dtype, device="cuda")
+
+            def call():
+                _native.fp8_gemm(a.data_ptr(), a.stride(0), sa.data_ptr(), sa.stride(0), sa.stride(1), w.data_ptr(),
+                                 w.stride(0), sw.data_ptr(), sw.stride(0), sw.stride(1), m, n, k, y[1:].data_ptr(),
+                                 ld, code, flag.data_ptr(), torch.cuda.current_stream().cuda_stream)
+
+            assert kernel in launches(call)[0].name
+            call()
+            check_product(y[1:m + 1, :n], a, sa, w, sw)
+            assert (y[0] == -7).all() and (y[m + 1] == -7).all() and (y[1:m + 1, n:] == -7).all()
+    assert not flag.any()
+
+
 # ------------------------------------------------------------------ scales and rows apart
 @pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (2500, 4200, 400, PAIRS)])
 def test_wide_rows_whose_scales_leave_the_range_beside_others(m, n, k, kernel):
