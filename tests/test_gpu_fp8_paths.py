@@ -8,11 +8,14 @@ import pytest
 import torch
 
 from cuda_launches import launches
-from fp8_reference import check_product
+from fp8_reference import BLOCK, check_product, check_quantized, e4m3
 
 pytestmark = pytest.mark.gpu
 
+FEW = {16: "few_rows_kernelILi16E", 32: "few_rows_kernelILi32E", 64: "few_rows_kernelILi64E"}
 WIDE, PAIRS = "wide_kernelILi1E", "wide_kernelILi2E"
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+NORM_REL = 2.0 ** -18  # test_gpu_fp8.py
 
 
 def rand(shape, seed, dtype=torch.float32, scale=1.0):
@@ -27,16 +30,107 @@ def operands(m, n, k, seed=0):
 
 
 def product(a, sa, w, sw, dtype, kernel, parts=1):
-    """fp8.gemm, which has to take `kernel` with every tile's K in `parts`."""
+    """fp8.gemm, which has to take `kernel` with every tile's K in `parts` (3: or more)."""
     from llvq_paper_reproduction_b200 import fp8
 
     y = fp8.gemm(a, sa, w, sw, out_dtype=dtype, check=True)
-    (launch,) = launches(lambda: fp8.gemm(a, sa, w, sw, out_dtype=dtype))
-    assert kernel in launch.name and launch.cluster == (2 if kernel == PAIRS else parts), launch
+    *_, launch = launches(lambda: fp8.gemm(a, sa, w, sw, out_dtype=dtype))  # behind copies of operands
+    assert kernel in launch.name, launch
+    assert launch.cluster == (2 if kernel == PAIRS else parts) or launch.cluster > parts > 2, launch
     return y
 
 
+# ------------------------------------------------------------------ the product's loops
+# CTA pairs: several tiles a pair, ragged in all three directions, K beyond the stage ring (5 blocks), the
+# first scale group (8) and the first use of both scale slots (16); rows of the output stored by TMA (4200),
+# in 8-byte words (bf16 4204, fp32 4202) and shifted (4201; bf16 4202)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(2500, 4200, 1000), (2500, 4201, 2200), (2500, 4202, 2200), (2500, 4204, 520),
+                                   (5003, 2500, 2304)])
+def test_pairs(m, n, k, dtype):
+    ops = operands(m, n, k)
+    check_product(product(*ops, dtype, PAIRS), *ops)
+
+
+# a tile per CTA, the same limits (its ring has 4 stages)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(250, 14336, 4096), (250, 14337, 4200), (600, 4100, 400), (1000, 4098, 2300)])
+def test_a_tile_per_cta(m, n, k, dtype):
+    ops = operands(m, n, k)
+    check_product(product(*ops, dtype, WIDE), *ops)
+
+
+# K of a tile in parts, which are added in both forms (two parts, and three or more) over whole and cut tiles
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,parts", [(512, 4096, 4096, 2), (500, 4099, 4000, 2), (256, 4096, 4096, 3),
+                                         (250, 4090, 4000, 3), (130, 4096, 14336, 3), (128, 3000, 14300, 3),
+                                         (128, 4097, 14300, 3)])
+def test_wide_tiles_with_k_in_parts(m, n, k, parts, dtype):
+    ops = operands(m, n, k)
+    check_product(product(*ops, dtype, WIDE, parts), *ops)
+
+
+# more blocks in a CTA than one chunk of scales holds (64, 32 and 16 of them)
+@pytest.mark.parametrize("m,rows,n,k", [(16, 16, 20000, 9000), (5, 16, 20001, 9000), (32, 32, 20000, 5000),
+                                        (64, 64, 28672, 4096), (50, 64, 20001, 6000)])
+def test_few_rows_with_several_chunks_of_scales(m, rows, n, k):
+    ops = operands(m, n, k)
+    check_product(product(*ops, torch.float32, FEW[rows]), *ops)
+
+
+@pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (2500, 4200, 400, PAIRS)])
+def test_wide_products_are_the_same_on_every_call_and_for_any_strides(m, n, k, kernel):
+    from llvq_paper_reproduction_b200 import fp8
+
+    a, sa, w, sw = operands(m, n, k)
+    want = product(a, sa, w, sw, torch.float32, kernel)
+    dense_a, dense_w = (t.view(torch.uint8).contiguous().view(fp8.E4M3) for t in (a, w))
+    wide = torch.full((m, 1040), 0x7F, dtype=torch.uint8, device="cuda")  # NaN beside the operand
+    wide[:, 16:16 + k] = dense_a.view(torch.uint8)
+    turned = dense_w.view(torch.uint8).t().contiguous().view(fp8.E4M3).t()
+    for b, sb, v, sv in ((a, sa, w, sw), (dense_a, sa.contiguous(), dense_w, sw.t().contiguous().t()),
+                         (wide.view(fp8.E4M3)[:, 16:16 + k], sa, turned, sw)):
+        assert torch.equal(want, product(b, sb, v, sv, torch.float32, kernel))
+    one = (dense_a[:1].expand(m, -1), sa[:1].expand(m, -1), w, sw)
+    check_product(fp8.gemm(*one, out_dtype=torch.float32, check=True), *one)
+
+
+@pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (512, 4096, 2000, WIDE), (2500, 4200, 400, PAIRS)])
+def test_wide_rows_that_are_not_finite_stay_in_their_rows(m, n, k, kernel):
+    from llvq_paper_reproduction_b200 import fp8
+
+    x, weight = rand((m, k), 20), fp8.quantize_blocks(rand((n, k), 21, scale=0.02))
+    want = fp8.gemm(*fp8.quantize_rows(x), *weight, out_dtype=torch.float32, check=True)
+    x[1, 300] = float("nan")
+    x[m - 2, k - 1] = float("inf")
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[[1, m - 2]] = True
+    q, s = fp8.quantize_rows(x)
+    got = fp8.gemm(q, s, *weight, out_dtype=torch.float32, check=True)
+    assert kernel in launches(lambda: fp8.gemm(q, s, *weight, out_dtype=torch.float32))[0].name
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
+
+
 # ------------------------------------------------------------------ the product's edges
+@pytest.mark.parametrize("m,n,k,kernel", [(3, 300, 500, FEW[16]), (30, 300, 1025, FEW[32]), (60, 300, 2200, FEW[64]),
+                                          (600, 4096, 500, WIDE), (256, 4096, 4003, WIDE), (2500, 4200, 1001, PAIRS)])
+def test_nothing_beside_the_columns_is_read_into_a_product(m, n, k, kernel):
+    """Rows of k columns with NaN behind them, in the same 16 bytes and further on."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    a, sa, w, sw = operands(m, n, k)
+
+    def between_nans(q):
+        held = torch.full((q.shape[0] + 1, q.stride(0) + 16), 0x7F, dtype=torch.uint8, device="cuda")
+        held[:-1, :k] = q.view(torch.uint8)
+        return held.view(fp8.E4M3)[:-1, :k]
+
+    want = fp8.gemm(a, sa, w, sw, out_dtype=torch.float32, check=True)
+    *_, launch = launches(lambda: fp8.gemm(between_nans(a), sa, between_nans(w), sw))
+    assert kernel in launch.name
+    assert torch.equal(want, fp8.gemm(between_nans(a), sa, between_nans(w), sw, out_dtype=torch.float32))
+
+
 @pytest.mark.parametrize("m,n,k,kernel", [(600, 4100, 300, WIDE), (500, 4099, 2000, WIDE), (2500, 4100, 300, PAIRS)])
 def test_wide_products_write_only_their_output(m, n, k, kernel):
     """Through the C ABI: an output inside a wider buffer, with what lies around it left as it was."""
@@ -134,6 +228,51 @@ def test_wide_rows_of_zeros_and_of_small_numbers(m, n, k, kernel):
     y = product(a, sa, w, sw * (2.0 ** -6 / sw.amax()), torch.float32, kernel)
     assert not y[~live].any() and y[live].isfinite().all()
     check_product(y, a, sa, w, sw * (2.0 ** -6 / sw.amax()))
+
+
+# ------------------------------------------------------------------ the norm's loop over rows
+# every CTA takes several rows: the next row ahead of or behind the barrier (up to 8192 columns), two
+# chunks (up to 16,384), two of 1024 threads, and rows on odd boundaries
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k", [(5000, 4096), (3000, 4100), (1500, 11008), (700, 20000), (2500, 4097), (1000, 11009),
+                                 (500, 20001)])
+def test_norm_of_several_rows_a_cta(m, k, residual, dtype):
+    from llvq_paper_reproduction_b200 import fp8
+
+    x, r = rand((m, k), 70, dtype, 2.0), rand((m, k), 71, dtype) if residual else None
+    w = (1 + 0.1 * rand((k,), 72)).to(dtype)
+    (launch,) = launches(lambda: fp8.rms_norm(x, w, residual=r))
+    assert "rms_norm_kernel" in launch.name and 2 * launch.grid < m, launch
+    for _ in range(2):
+        out = fp8.rms_norm(x, w, residual=r)
+        h = x.double() + (r.double() if residual else 0)
+        y = h * w.double() / torch.sqrt(h.square().mean(dim=1, keepdim=True) + 1e-5)
+        check_quantized(out[0], out[1], y, 1, NORM_REL)
+        assert not residual or torch.equal(out[2], (x.float() + r.float()).to(dtype))
+        x.copy_(x.flip(0))  # other rows for every CTA
+
+
+# ------------------------------------------------------------------ ties
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(900, 4096), (301, 1030), (140, 4099)])
+def test_bytes_of_16_bit_inputs_are_the_rounded_quotient(shape, dtype):
+    """448 x / amax of 16-bit numbers is a tie of e4m3 or at least 2^-16 of
+    itself away from one, so the nearest byte is one and no other.  In 64 bits 448 x is exact
+    and the quotient of a tie is the tie, so the reference's rounding is right."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    x = rand(shape, 73, dtype)
+    x[:, 5::BLOCK] = 7.0  # amax a multiple of 7: ties by the dozen
+    m, k = shape
+    for f, rows in ((fp8.quantize_rows, 1), (fp8.quantize_blocks, BLOCK)):
+        q, _ = f(x)
+        p = torch.nn.functional.pad(x.double(), (0, -k % BLOCK, 0, -m % rows))
+        p = p.view(-1, rows, p.shape[1] // BLOCK, BLOCK)
+        want = 448.0 * p / p.abs().amax(dim=(1, 3), keepdim=True)
+        ties = (want / torch.exp2(torch.frexp(want)[1].clamp(min=-5).double() - 5)).remainder(2.0) == 1.0
+        assert ties.sum() > 100
+        assert torch.equal(q.double(), e4m3(want).view(-1, p.shape[2] * BLOCK)[:m, :k])
 
 
 # ------------------------------------------------------------------ what a call may be given
