@@ -227,7 +227,7 @@ int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_
  * correctly rounded there) and rounded to even.  NaN makes its whole block NaN; an infinity makes
  * the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
  * have a stride in elements, e4m3 rows start on 16-byte boundaries (base and
- * stride).  Outputs must not overlap inputs.  Device: the current one.  Nothing is allocated and no call
+ * stride), everything else on its elements'.  Outputs must not overlap inputs.  Device: the current one.  Nothing is allocated and no call
  * keeps state, so calls may overlap on any streams and be captured. */
 
 /* x [rows, cols] -> q, scales of 1 x 128 blocks (block_rows = 1, activations)

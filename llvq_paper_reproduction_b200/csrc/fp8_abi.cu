@@ -15,12 +15,16 @@ namespace {
 
 bool known_type(int32_t t) { return t == LLVQ_DT_F32 || t == LLVQ_DT_F16 || t == LLVQ_DT_BF16; }
 bool on_boundary(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// Elements of a type lie on their own boundary (an access off it would fault).
+bool elements_at(const void* p, int32_t type) { return on_boundary(p, type == LLVQ_DT_F32 ? 4 : 2); }
+constexpr const char* kOffBoundary = "an address is off its elements' boundary";
 
 // Outputs of a quantizer over [rows, cols].
 const char* bad_out(const uint8_t* q, int64_t ldq, const float* scale, int64_t rows, int64_t cols) {
   if (rows == 0 || cols == 0) return nullptr;
   if (!q || !scale) return "null output";
   if (rows > llvq::kFp8MaxUnits / ((cols - 1) / llvq::kFp8Block + 1)) return "more than 2^32 - 2^16 blocks";
+  if (!on_boundary(scale, 4)) return kOffBoundary;
   if (ldq < cols || ldq % 16 || !on_boundary(q, 16)) return "e4m3 rows must be 16-byte aligned (base and stride)";
   return nullptr;
 }
@@ -35,6 +39,7 @@ int llvq_fp8_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t rows, 
     return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_quantize: bad size, type or block (1 or 128 rows)");
   if (const char* why = bad_out(q, ldq, scale, rows, cols)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, why);
   if (rows > 0 && cols > 0 && !x) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_quantize: null input");
+  if (!elements_at(x, x_type)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, kOffBoundary);
   const cudaError_t e = llvq::fp8_quantize_launch({x, ldx}, x_type, rows, cols, block_rows,
                                                   {q, ldq, scale, scale_row, scale_col}, (cudaStream_t)stream);
   return e == cudaSuccess ? LLVQ_OK : abi_cuda_error(e, "fp8_quantize launch");
@@ -47,6 +52,7 @@ int llvq_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t l
     return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_swiglu: bad size or type");
   if (const char* why = bad_out(q, ldq, scale, rows, cols)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, why);
   if (rows > 0 && cols > 0 && (!gate || !up)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_swiglu: null input");
+  if (!elements_at(gate, type) || !elements_at(up, type)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, kOffBoundary);
   const cudaError_t e = llvq::fp8_swiglu_launch({gate, ld_gate}, {up, ld_up}, type, rows, cols,
                                                 {q, ldq, scale, scale_row, scale_col}, (cudaStream_t)stream);
   return e == cudaSuccess ? LLVQ_OK : abi_cuda_error(e, "fp8_swiglu launch");
@@ -67,6 +73,9 @@ int llvq_fp8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t 
   if (const char* why = bad_out(q, ldq, scale, rows, cols)) return abi_error(LLVQ_ERR_INVALID_ARGUMENT, why);
   if (rows > 0 && cols > 0 && (!x || !weight || (!residual != !hidden)))
     return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_rms_norm: null pointer (residual and hidden come together)");
+  if (!elements_at(x, type) || !elements_at(residual, type) || !elements_at(hidden, type) ||
+      !elements_at(weight, weight_type))
+    return abi_error(LLVQ_ERR_INVALID_ARGUMENT, kOffBoundary);
   const cudaError_t e =
       llvq::fp8_rms_norm_launch({x, ldx}, {residual, ld_residual}, type, weight, weight_type, eps, rows, cols, hidden,
                                 ld_hidden, {q, ldq, scale, scale_row, scale_col}, (cudaStream_t)stream);
@@ -86,6 +95,9 @@ int llvq_fp8_gemm(const uint8_t* a, int64_t lda, const float* a_scale, int64_t a
     return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_gemm: null pointer");
   if (k > 0 && (lda < k || ldw < k || lda % 16 || ldw % 16 || !on_boundary(a, 16) || !on_boundary(w, 16)))
     return abi_error(LLVQ_ERR_INVALID_ARGUMENT, "fp8_gemm: e4m3 rows must be 16-byte aligned (base and stride)");
+  if (!elements_at(y, y_type) || !on_boundary(error_flag, 4) ||
+      (k > 0 && (!on_boundary(a_scale, 4) || !on_boundary(w_scale, 4))))
+    return abi_error(LLVQ_ERR_INVALID_ARGUMENT, kOffBoundary);
   const cudaError_t e =
       llvq::fp8_gemm_launch({a, lda, a_scale, a_scale_row, a_scale_col}, {w, ldw, w_scale, w_scale_row, w_scale_col},
                             m, n, k, y, ldy, y_type, error_flag, (cudaStream_t)stream);

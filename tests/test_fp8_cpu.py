@@ -85,3 +85,23 @@ def test_c_entries_take_empty_calls():
     _native.fp8_gemm(0, 0, 0, 1, 1, 0, 0, 0, 1, 1, 0, 4, 128, 0, 4, 0, 0, 0)
     _native.fp8_gemm(0, 0, 0, 1, 1, 0, 0, 0, 1, 1, 4, 0, 128, 0, 0, 0, 0, 0)
 
+
+
+@pytest.mark.parametrize("call", [
+    lambda: _native.fp8_quantize(P + 2, 0, 128, 1, 128, 1, P, 128, P, 1, 1, 0),
+    lambda: _native.fp8_quantize(P + 1, 2, 128, 1, 128, 1, P, 128, P, 1, 1, 0),
+    lambda: _native.fp8_quantize(P, 2, 128, 1, 128, 1, P, 128, P + 2, 1, 1, 0),                       # scale
+    lambda: _native.fp8_swiglu(P, 128, P + 1, 128, 1, 1, 128, P, 128, P, 1, 1, 0),                    # up
+    lambda: _native.fp8_swiglu(P + 2, 128, P, 128, 0, 1, 128, P, 128, P, 1, 1, 0),                    # gate
+    lambda: _native.fp8_rms_norm(P, 128, 0, 0, 1, P + 2, 0, 1e-5, 1, 128, 0, 0, P, 128, P, 1, 1, 0),  # fp32 weight
+    lambda: _native.fp8_rms_norm(P, 128, P + 1, 128, 1, P, 1, 1e-5, 1, 128, P, 128, P, 128, P, 1, 1, 0),  # residual
+    lambda: _native.fp8_rms_norm(P, 128, P, 128, 1, P, 1, 1e-5, 1, 128, P + 1, 128, P, 128, P, 1, 1, 0),  # hidden
+    lambda: _native.fp8_gemm(P, 128, P + 1, 1, 1, P, 128, P, 1, 1, 4, 4, 128, P, 4, 0, 0, 0),         # a's scales
+    lambda: _native.fp8_gemm(P, 128, P, 1, 1, P, 128, P + 2, 1, 1, 4, 4, 128, P, 4, 0, 0, 0),         # w's scales
+    lambda: _native.fp8_gemm(P, 128, P, 1, 1, P, 128, P, 1, 1, 4, 4, 128, P + 2, 4, 0, 0, 0),         # fp32 output
+    lambda: _native.fp8_gemm(P, 128, P, 1, 1, P, 128, P, 1, 1, 4, 4, 128, P + 1, 4, 2, 0, 0),         # bf16 output
+    lambda: _native.fp8_gemm(P, 128, P, 1, 1, P, 128, P, 1, 1, 4, 4, 128, P, 4, 2, P + 2, 0),         # error flag
+])
+def test_c_entries_refuse_addresses_off_their_elements_boundary(call):
+    with pytest.raises(ValueError, match="boundary"):
+        call()
