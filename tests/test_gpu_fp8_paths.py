@@ -70,6 +70,15 @@ def test_wide_tiles_with_k_in_parts(m, n, k, parts, dtype):
     check_product(product(*ops, dtype, WIDE, parts), *ops)
 
 
+# many rows of next to nothing, and a vocabulary's worth of columns
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,kernel", [(20000, 8, 300, PAIRS), (20000, 1, 130, PAIRS), (20001, 300, 1, PAIRS),
+                                          (10000, 5, 130, WIDE), (10001, 16, 16, WIDE), (3, 128300, 600, FEW[16])])
+def test_narrow_and_shallow_products(m, n, k, kernel, dtype):
+    ops = operands(m, n, k)
+    check_product(product(*ops, dtype, kernel), *ops)
+
+
 # more blocks in a CTA than one chunk of scales holds (64, 32 and 16 of them)
 @pytest.mark.parametrize("m,rows,n,k", [(16, 16, 20000, 9000), (5, 16, 20001, 9000), (32, 32, 20000, 5000),
                                         (64, 64, 28672, 4096), (50, 64, 20001, 6000)])
