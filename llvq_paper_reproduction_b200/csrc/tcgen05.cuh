@@ -1,5 +1,5 @@
-// Thin inline-PTX wrappers for the sm_100a tensor-core path of the
-// dequant-GEMM: TMEM allocation, tcgen05.mma (kind::f16, operands in shared
+// Thin inline-PTX wrappers for the sm_100a tensor-core paths of the
+// dequant-GEMM and the 8-bit product: TMEM allocation, tcgen05.mma (operands in shared
 // memory), tcgen05.commit to an mbarrier, TMEM -> register loads, TMA tile
 // loads (no multicast), mbarrier arrivals and bounded mbarrier waits.
 #pragma once
@@ -176,20 +176,7 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t
       : "memory");
 }
 
-// 32 lanes x 32 consecutive fp32 columns of TMEM; the values are there after tmem_wait_ld().
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-
-// The same of 64 columns.
+// 32 lanes x 64 consecutive fp32 columns of TMEM; the values are there after tmem_wait_ld().
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
