@@ -223,9 +223,10 @@ int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_
  * its block; the last block of a row may be partial.  Scales lie anywhere:
  * scale[r * scale_row + b * scale_col] for row (or row block) r and column
  * block b.  For each block amax = max(2^-100, max |y|), scale = amax / 448,
- * byte = e4m3(448 y / amax), formed in fp32 (the quantizer's quotient is
- * correctly rounded there) and rounded to even.  NaN makes its whole block NaN; an infinity makes
- * the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
+ * byte = e4m3(448 y / amax), the quotient formed in fp32 (by the quantizers exact
+ * where it is a tie of 16-bit inputs, so that their bytes are the correctly
+ * rounded ones; within 2^-23 of fp32 inputs') and rounded to even.  NaN makes its
+ * whole block NaN; an infinity makes the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
  * have a stride in elements, e4m3 rows start on 16-byte boundaries (base and
  * stride), everything else on its elements'.  Outputs must not overlap inputs.  Device: the current one.  Nothing is allocated and no call
  * keeps state, so calls may overlap on any streams and be captured. */
@@ -253,7 +254,7 @@ int llvq_fp8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t 
  * sum_{k in b} a[m, k] w[n, k]: each block's sum on the tensor cores, scaled
  * and added in fp32, rounded once to y_type.  a [m, k] with 1 x 128 scales, w
  * [n, k] with 128 x 128 scales; y has row stride ldy.  k = 0 gives zeros.  One summation order
- * per output and shape.  *error_flag (device int, may be NULL) is set to 1 if
+ * per output, shape and GPU (its SMs decide how K is split).  *error_flag (device int, may be NULL) is set to 1 if
  * a tensor-core wait timed out. */
 int llvq_fp8_gemm(const uint8_t* a, int64_t lda, const float* a_scale, int64_t a_scale_row, int64_t a_scale_col,
                   const uint8_t* w, int64_t ldw, const float* w_scale, int64_t w_scale_row, int64_t w_scale_col,

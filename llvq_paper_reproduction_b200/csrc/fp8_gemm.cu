@@ -399,8 +399,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 // the leader's acc_empty[] takes the arrivals of all 16 adding warps.
 //
 // What bounds it: a block costs about 860 cycles where its MMAs take 512
-// (4096 x 14336 x 4096: 219 us, 2.2 PFLOP/s; without the additions 191, without
-// the TMEM loads too 176).  An adding warp's pass is a chain of latencies: the
+// (4096 x 14336 x 4096 in a captured graph at 1.69 GHz: 219 us, 2.2 PFLOP/s; without
+// the additions 191, without the TMEM loads too 176; call after call, at the
+// 1.48 GHz of the power limit, 257 us, 1.87 PFLOP/s).  Beside that pairs idle where the
+// tiles leave their last round partly empty: 896 tiles there, 13 rounds for the work of 12.1;
+// 1280 x 4096, 80 tiles, two rounds for 1.08.  An adding warp's pass is a chain of latencies: the
 // block's sums ready, a TMEM load, 32 FFMA2, a second load, the buffer handed
 // back, 32 FFMA2 (2.4 cycles each on a scheduler); hence loads of 64 columns, and
 // the look for the next block before the last additions.  Measured beside it:

@@ -5,8 +5,8 @@
 // For a block B of values y (1 x 128 columns, or 128 x 128 for weights):
 //   amax = max(2^-100, max |y|)      scale = amax / 448      q = e4m3(448 y / amax)
 // 448 is the largest e4m3 value, so nothing saturates; the quotient is formed in
-// fp32 (correctly rounded by the quantizers, as one product with 448 / amax by
-// norm and gate, whose y carry roundings already) and rounded to even.  NaN in
+// fp32 (by the quantizers with a residual step, by norm and gate, whose y carry
+// roundings already, as one product with 448 / amax) and rounded to even.  NaN in
 // a block makes amax, hence the whole block, NaN; an infinity makes scale
 // infinite, its own value NaN and the others 0.  The floor 2^-100 keeps the
 // reciprocal finite: blocks below it (zeros above all) give q = 0 or values
@@ -164,8 +164,8 @@ __device__ __forceinline__ void store_vec(T* p, const Raw<T>& r, int valid) {
 // columns in loads and stores of one element a lane, neighbours side by side, turned
 // through 1 KB of the warp's shared memory into sixteen elements a thread and back.
 // (Loads of a thread's own columns touched 32 sectors each: 8000 x 4097 bf16 norm
-// with a residual 216 us against 84, rows 47 against 24, gate 79 against 44,
-// 128 x 128 blocks 38 against 26.)
+// with a residual 216 us against 84, rows 47 against 24, gate 79 against 42,
+// 128 x 128 blocks 38 against 27.)
 // unit(u, &left): block u's first element and its columns in the matrix, 0..128.
 constexpr int kTurnBytes = 1024;
 
@@ -308,7 +308,7 @@ __device__ __forceinline__ float inverse_root(float v) {
 }
 
 // 448 v / amax for values v that fp32 holds exactly: q0 = z r with z = 448 v
-// (exact for 16-bit inputs) and r = 1 / amax, and one residual step, q = q0 +
+// (exact for 16-bit inputs; of fp32 ones a rounding of 2^-24, which q keeps beside its own) and r = 1 / amax, and one residual step, q = q0 +
 // (z - q0 amax) r (Markstein 1990).  Inputs of few bits lie on ties of e4m3
 // often, and there the residual is exact and q is the tie itself, so that it
 // is rounded to even as it should; a quotient off by one unit would fall on
@@ -418,7 +418,7 @@ __device__ __forceinline__ F2 silu(F2 g) {
 // fp32's normal range there, and the product need not.  1 + exp(-gate) is
 // exp(-gate) to the last bit, so with E = exp(gate / 2) it is (gate E) (E up).  E
 // is 0 below gate = -174.7, where the product is below 2^-116 whatever up is.  A
-// group of sixteen asks for its smallest gate first: 64 x 14336 bf16 3.3 us, 3.1
+// group of sixteen asks for its smallest gate first: 64 x 14336 bf16 3.2 us, 3.1
 // without.
 constexpr float kLowGate = -87.f;
 __device__ __forceinline__ F2 low_gate(F2 gate, F2 up) {
@@ -639,7 +639,9 @@ __global__ void __launch_bounds__(kBlockThreads) blocks_kernel(const T* x, int64
 // threads, which leave no registers for it.  (Rows on odd boundaries: norm_typed.)  (One chunk of 688 threads, for 11008
 // columns, left an SM with a single CTA: 63 us against the two chunks' 58 for
 // 4096 rows.)  8192 x 4096 with a residual runs at 6.3 TB/s.
-// Registers a thread: as few as leave nothing, or little, spilled.
+// Registers a thread.  Nothing is spilled (8 bytes for fp32 above 16,384 columns
+// with a residual) where vectors are loaded; rows on odd boundaries spill up to 408 bytes at
+// 16,384 columns at most and 256 to 1416 beyond, where 1024 threads leave 64 registers each.
 constexpr int norm_regs(int chunks, int threads, int step) {
   return threads == 1024 ? 64 : chunks == 2 ? 88 : step == 1 ? 80 : 64;
 }

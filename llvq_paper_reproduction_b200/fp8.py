@@ -61,7 +61,8 @@ _ext = _load()
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [rows, cols] -> (q, scale [rows, ceil(cols / 128)]): per block of 128
     columns amax = max(2^-100, max |x|), scale = amax / 448 and
-    q = e4m3(448 x / amax), rounded to nearest even.  NaN makes its block NaN;
+    q = e4m3(448 x / amax), rounded to nearest even: the right byte for every 16-bit
+    x; of fp32 the quotient is rounded to fp32 first (within 2^-23).  NaN makes its block NaN;
     an infinity makes the block's scale infinite."""
     return _ext.quantize_rows(x)
 
@@ -95,8 +96,8 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     [m, ceil(k / 128)]) and an 8-bit weight (w [n, k], w_scale
     [ceil(n / 128), ceil(k / 128)]): the tensor cores sum each block of 128
     columns, the sums are scaled and added in fp32 and rounded once to
-    out_dtype (bfloat16, float16 or float32).  One summation order per output
-    and shape: the same bits on every call.  Scales may have any strides; 8-bit
+    out_dtype (bfloat16, float16 or float32).  One summation order per output,
+    shape and GPU: the same bits on every call.  Scales may have any strides; 8-bit
     rows that do not start on 16-byte boundaries are copied.  Asynchronous: a
     tensor-core wait that timed out is counted in ``pending_errors``;
     ``check=True`` synchronises and raises RuntimeError at once (not while a

@@ -252,7 +252,10 @@ class LeechLatticeVectorQuantizerGpu:
         padding of the last block off (default: all 24 * blocks columns).
         Against the dequant-GEMM it takes a byte instead of 2 bits per weight
         and rounds the weight to 3 fraction bits, and gives large batches
-        the 8-bit tensor rate.  Errors as in ``dequantize_bf16``.  No
+        the 8-bit tensor rate.  The weight passes through a bf16 matrix.  Of a
+        weight quantized under a rotation this is the rotated weight: its
+        activations have to be rotated before they are quantized (``gemm``'s
+        ``rotation`` has no counterpart here).  Errors as in ``dequantize_bf16``.  No
         reference counterpart."""
         from . import fp8
 
