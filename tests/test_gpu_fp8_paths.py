@@ -87,6 +87,30 @@ def test_few_rows_with_several_chunks_of_scales(m, rows, n, k):
     check_product(product(*ops, torch.float32, FEW[rows]), *ops)
 
 
+def test_products_of_every_kind_at_once():
+    """On five streams, so that CTAs of different kernels share SMs and their
+    tensor memory: the same bits as one after the other."""
+    from llvq_paper_reproduction_b200 import fp8
+
+    sizes = [(2500, 4200, 1000, PAIRS), (256, 4096, 4096, WIDE), (600, 4100, 400, WIDE), (5, 20001, 2000, FEW[16]),
+             (64, 4096, 8000, FEW[64])]
+    ops = [operands(m, n, k, i) for i, (m, n, k, _) in enumerate(sizes)]
+    want = [fp8.gemm(*o) for o in ops]
+    for o, (*_, kernel) in zip(ops, sizes):
+        assert kernel in launches(lambda: fp8.gemm(*o))[0].name
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sizes]
+    got = [[] for _ in sizes]
+    for _ in range(12):
+        for i, (o, s) in enumerate(zip(ops, streams)):
+            with torch.cuda.stream(s):
+                got[i] += [fp8.gemm(*o) for _ in range(1 + i)]
+    torch.cuda.synchronize()
+    fp8.raise_pending_errors()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(w, y) for y in ys)
+
+
 @pytest.mark.parametrize("m,n,k,kernel", [(600, 4096, 400, WIDE), (2500, 4200, 400, PAIRS)])
 def test_wide_products_are_the_same_on_every_call_and_for_any_strides(m, n, k, kernel):
     from llvq_paper_reproduction_b200 import fp8
