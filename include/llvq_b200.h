@@ -226,10 +226,12 @@ int llvq_rotate_scale(const uint16_t* in_f16, int64_t rows, int64_t cols, int64_
  * byte = e4m3(448 y / amax), the quotient formed in fp32 (by the quantizers exact
  * where it is a tie of 16-bit inputs, so that their bytes are the correctly
  * rounded ones; within 2^-23 of fp32 inputs') and rounded to even.  NaN makes its
- * whole block NaN; an infinity makes the scale infinite and its own byte NaN.  Types are LLVQ_DT_*; input rows
- * have a stride in elements, e4m3 rows start on 16-byte boundaries (base and
- * stride), everything else on its elements'.  Outputs must not overlap inputs.  Device: the current one.  Nothing is allocated and no call
- * keeps state, so calls may overlap on any streams and be captured. */
+ * whole block NaN; an infinity makes the scale infinite and its own byte NaN.
+ * Types are LLVQ_DT_*; input rows have a stride in elements, e4m3 rows start on
+ * 16-byte boundaries (base and stride), everything else on its elements'.
+ * Outputs must not overlap inputs.  Device: the current one.  Nothing is
+ * allocated and no call keeps state, so calls may overlap on any streams and be
+ * captured. */
 
 /* x [rows, cols] -> q, scales of 1 x 128 blocks (block_rows = 1, activations)
  * or 128 x 128 blocks (block_rows = 128, weights). */
@@ -253,9 +255,10 @@ int llvq_fp8_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t 
 /* y[m, n] = sum over column blocks b of a_scale[m, b] w_scale[n / 128, b] *
  * sum_{k in b} a[m, k] w[n, k]: each block's sum on the tensor cores, scaled
  * and added in fp32, rounded once to y_type.  a [m, k] with 1 x 128 scales, w
- * [n, k] with 128 x 128 scales; y has row stride ldy.  k = 0 gives zeros.  One summation order
- * per output, shape and GPU (its SMs decide how K is split).  *error_flag (device int, may be NULL) is set to 1 if
- * a tensor-core wait timed out. */
+ * [n, k] with 128 x 128 scales; y has row stride ldy and nothing but its [m, n]
+ * is written.  k = 0 gives zeros.  One summation order per output, shape and GPU
+ * (its SMs decide how K is split).  *error_flag (device int, may be NULL) is set
+ * to 1 if a tensor-core wait timed out. */
 int llvq_fp8_gemm(const uint8_t* a, int64_t lda, const float* a_scale, int64_t a_scale_row, int64_t a_scale_col,
                   const uint8_t* w, int64_t ldw, const float* w_scale, int64_t w_scale_row, int64_t w_scale_col,
                   int64_t m, int64_t n, int64_t k, void* y, int64_t ldy, int32_t y_type, int32_t* error_flag,

@@ -437,8 +437,8 @@ struct Wide {
 // acc + v * (as ws).  Where that product is below fp32's normal numbers or not
 // finite (plain false), the two are applied one after the other; by the lane, so
 // that no row depends on another.  A normal product is rounded once, wherever it
-// lies: rows of zeros, whose scale is the floor's 2^-108.8, stay on the plain side (400 x
-// 14336 x 4096 with a quarter of the rows zero: 35.4 us; 42.7 when 2^-60 was the end).
+// lies: rows of zeros, whose scale is the floor's 2^-108.8, stay on the plain side
+// (400 x 14336 x 4096 with a quarter of the rows zero: 35.4 us; 42.7 when 2^-60 was the end).
 struct Scale {
   float factor, pre;
   bool plain;

@@ -308,8 +308,9 @@ __device__ __forceinline__ float inverse_root(float v) {
 }
 
 // 448 v / amax for values v that fp32 holds exactly: q0 = z r with z = 448 v
-// (exact for 16-bit inputs; of fp32 ones a rounding of 2^-24, which q keeps beside its own) and r = 1 / amax, and one residual step, q = q0 +
-// (z - q0 amax) r (Markstein 1990).  Inputs of few bits lie on ties of e4m3
+// (exact for 16-bit inputs; fp32 ones carry a rounding of 2^-24 from here on) and
+// r = 1 / amax, and one residual step, q = q0 + (z - q0 amax) r (Markstein 1990).
+//  Inputs of few bits lie on ties of e4m3
 // often, and there the residual is exact and q is the tie itself, so that it
 // is rounded to even as it should; a quotient off by one unit would fall on
 // either side.  448 and amax are both taken times 2^-64 where 448 amax could
@@ -496,10 +497,9 @@ template <typename T, bool kGated, int kStep>
 constexpr int kRowCtas = !kGated || kStep == 1 ? 0 : sizeof(T) == 4 ? 5 : 4;
 
 template <typename T, bool kGated, int kStep>
-__global__ void __launch_bounds__(kRowThreads, kRowCtas<T, kGated, kStep>) rows_kernel(const T* x, int64_t ldx, const T* up,
-                                                           int64_t ldu, uint32_t rows,
-                                                           uint32_t blocks, uint32_t skip_rows, uint32_t skip_blocks,
-                                                           int64_t cols, Fp8Out out) {
+__global__ void __launch_bounds__(kRowThreads, kRowCtas<T, kGated, kStep>)
+    rows_kernel(const T* x, int64_t ldx, const T* up, int64_t ldu, uint32_t rows, uint32_t blocks, uint32_t skip_rows,
+                uint32_t skip_blocks, int64_t cols, Fp8Out out) {
   dependents_may_start();
   constexpr int kUnits = kRowUnits<T, kGated, kStep>;
   constexpr int kTeams = kRowThreads / kGroup;
